@@ -20,6 +20,9 @@ DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
 NO_SLOT = -(1 << 63)                 # M355_NO_SLOT (include/mi355attn.h): out_cache_loc of a token without a slot
 PLAN_ERROR_WORD = 6                  # M355_PLAN_ERROR_WORD
 
+TREE_MAX_NODES = 1024                # M355_TREE_MAX_NODES
+MAX_TOP_LOGPROBS = 64                # M355_MAX_TOP_LOGPROBS
+
 MAX_RANKS = 8                        # M355_MAX_RANKS (include/mi355tp.h)
 
 
@@ -80,6 +83,20 @@ SIGNATURES = {
     "m355_rope_kv_store": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
                                      c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int32, c_int32,
                                      c_int64, c_int32, c_void_p]),
+    "m355_scored_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "m355_scored_attn": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int32, c_int32,
+                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32,
+                                   c_int32, c_int32, c_int32, c_int32, c_float, c_float, c_void_p, c_int32, c_void_p, c_void_p,
+                                   c_void_p, c_int64, c_int32, c_void_p]),
+    "m355_tree_prepare": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_int32, c_int32, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
+    "m355_tree_attn": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int32, c_int32,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int32, c_int32,
+                                 c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_float, c_void_p, c_void_p, c_int64,
+                                 c_int32, c_void_p]),
+    "m355_token_logprobs_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32]),
+    "m355_token_logprobs": (c_int32, [c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p]),
 }
 
 _lib = None

@@ -4,6 +4,9 @@ Every argument tensor must be on the GPU; results are enqueued on torch's curren
 """
 from __future__ import annotations
 
+import math
+from typing import NamedTuple, Optional
+
 import torch
 
 from . import _lib
@@ -382,3 +385,225 @@ def rope_kv_store(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, hea
                                  _ptr(k_pool), _ptr(v_pool), pool_pitch(k_pool, v_pool) if store else 0,
                                  _ptr(loc) if store else None, T, Hq, Hkv, D, S,
                                  dtype_code(q.dtype), current_stream()), "m355_rope_kv_store")
+
+
+# ---- attention with modified scores, trees of drafted tokens, log probabilities -----------------------------------------
+def _device_of(tensors) -> None:
+    """Every tensor on the GPU that is current: the launch goes to its stream, and kernels of one device must not be handed
+    another's memory."""
+    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for n, t in tensors:
+        require_cuda(t, n)
+        if t.device.index != dev:
+            raise _lib.MI355AttnError(f"{n} is on {t.device}, the current device is cuda:{dev} (use torch.cuda.device)")
+
+
+def _vector(name: str, t, dtype, n: int) -> None:
+    if t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise _lib.MI355AttnError(f"{name} must be a contiguous {dtype} vector of {n}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _scored_buffers(what: str, q, k_pool, v_pool, page_table, num_heads: int, page_size: int, out, workspace, need: int):
+    """Shapes, types and strides that both scored entry points share.  Returns (q rows, pool pitch, out, workspace)."""
+    if k_pool.dim() != 3 or q.dim() < 2:
+        raise _lib.MI355AttnError(f"{what}: q must be [T, heads*D], the pools [S, Hkv, D]")
+    S, Hkv, D = k_pool.shape
+    T = q.shape[0]
+    if q.dtype != k_pool.dtype or q.dtype != v_pool.dtype:
+        raise _lib.MI355AttnError(f"{what}: q and the pools must have one dtype, got {q.dtype}, {k_pool.dtype}, {v_pool.dtype}")
+    if num_heads <= 0 or num_heads % Hkv or q.numel() != T * num_heads * D:
+        raise _lib.MI355AttnError(f"{what}: q {tuple(q.shape)} is not [T, {num_heads} * {D}], a multiple of {Hkv} kv heads")
+    q2 = q.reshape(T, num_heads * D)
+    if T and (q2.stride(1) != 1 or q2.stride(0) % 8 or q2.data_ptr() % 16):
+        q2 = q2.contiguous()
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 or page_size < 1:
+        raise _lib.MI355AttnError(f"{what}: page_table must be int32 [rows, pages] with inner stride 1, page_size >= 1")
+    if out is None:
+        out = torch.empty((T, num_heads * D), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or tuple(out.shape) != (T, num_heads * D) or (T and out.stride(1) != 1):
+        raise _lib.MI355AttnError(f"{what}: out must be {q.dtype} [T, heads*D] with inner stride 1")
+    elif T and out.data_ptr() == q2.data_ptr():
+        raise _lib.MI355AttnError(f"{what}: out must not be q")
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    elif not workspace.is_contiguous():
+        raise _lib.MI355AttnError(f"{what}: workspace must be contiguous")
+    return q2, pool_pitch(k_pool, v_pool), out, workspace
+
+
+def _stride0(t, width: int) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(width, t.stride(0))
+
+
+def scored_workspace_bytes(B: int, T: int, Hq: int, Hkv: int, D: int, max_extend_len: int, max_seq_len: int, window: int = 0) -> int:
+    return int(_lib.load().m355_scored_workspace_bytes(B, T, Hq, Hkv, D, max_extend_len, max_seq_len, window))
+
+
+def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
+                page_table_ids: torch.Tensor, seq_lens: torch.Tensor, page_size: int, num_heads: int, max_seq_len: int, *,
+                prefix_lens: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None, max_extend_len: int = 1,
+                softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, window: int = 0,
+                doc_starts: Optional[torch.Tensor] = None, bidir_lens: Optional[torch.Tensor] = None,
+                scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention over the paged pools whose scores are capped (softcap: x -> softcap * tanh(x / softcap)), biased by distance
+    (slopes, fp32 [Hq]: x -= slope * |pos - key|) or masked: a sliding window of `window` keys, doc_starts int32 [T] (where the
+    row's document begins) and bidir_lens int32 [B] (a prompt prefix visible to every row of its request).  Everything combines
+    (m355_scored_attn, include/mi355attn.h).
+
+    With prefix_lens (int64 [B]) and cu_q (int32 [B+1]): ragged rows over cached prefixes, as prefill_attn; rows of q at or past
+    cu_q[B] are left as they were in `out`.  Without them: one row per request, its newest token at seq_lens - 1.  A row that
+    sees nothing gives zeros."""
+    lib = _lib.load()
+    given = [("q", q), ("k_pool", k_pool), ("v_pool", v_pool), ("page_table", page_table), ("page_table_ids", page_table_ids),
+             ("seq_lens", seq_lens)]
+    given += [(n, t) for n, t in (("prefix_lens", prefix_lens), ("cu_q", cu_q), ("slopes", slopes), ("doc_starts", doc_starts),
+                                  ("bidir_lens", bidir_lens), ("workspace", workspace), ("out", out)) if t is not None]
+    _device_of(given)
+    B, T = seq_lens.numel(), q.shape[0]
+    if (prefix_lens is None) != (cu_q is None):
+        raise _lib.MI355AttnError("scored_attn: prefix_lens and cu_q go together (neither: one row per request)")
+    _vector("seq_lens", seq_lens, torch.int64, B), _vector("page_table_ids", page_table_ids, torch.int64, B)
+    if cu_q is not None:
+        _vector("prefix_lens", prefix_lens, torch.int64, B), _vector("cu_q", cu_q, torch.int32, B + 1)
+    elif T != B:
+        raise _lib.MI355AttnError(f"scored_attn: {T} rows for {B} requests (pass prefix_lens and cu_q for more than one row each)")
+    if slopes is not None:
+        _vector("slopes", slopes, torch.float32, num_heads)
+    if doc_starts is not None:
+        _vector("doc_starts", doc_starts, torch.int32, T)
+    if bidir_lens is not None:
+        _vector("bidir_lens", bidir_lens, torch.int32, B)
+    if cu_q is None:
+        max_extend_len = 1
+    D = k_pool.shape[-1]
+    need = scored_workspace_bytes(B, T, num_heads, k_pool.shape[1], D, max_extend_len, max_seq_len, window) if workspace is None else 0
+    q2, pitch, out, workspace = _scored_buffers("scored_attn", q, k_pool, v_pool, page_table, num_heads, page_size, out, workspace, need)
+    W = num_heads * D
+    check(lib.m355_scored_attn(q2.data_ptr(), _stride0(q2, W), k_pool.data_ptr(), v_pool.data_ptr(), pitch, k_pool.shape[0],
+                               page_table.data_ptr(), _stride0(page_table, page_table.shape[1]), page_table.shape[0], page_table.shape[1],
+                               page_table_ids.data_ptr(), seq_lens.data_ptr(), _ptr(prefix_lens), _ptr(cu_q), out.data_ptr(),
+                               _stride0(out, W), B, T, max_extend_len, max_seq_len, num_heads, k_pool.shape[1], D, page_size,
+                               float(D) ** -0.5 if scale is None else scale, softcap, _ptr(slopes), window, _ptr(doc_starts),
+                               _ptr(bidir_lens), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+                               dtype_code(q.dtype), current_stream()), "m355_scored_attn")
+    return out
+
+
+class TreePlan(NamedTuple):
+    """What tree_prepare makes once per verification step, for every layer's tree_attn."""
+    mask: torch.Tensor                 # int32 [T, words]: bit x of word w = node 32 w + x is the row's node or an ancestor
+    positions: torch.Tensor            # int64 [T]: prefix + depth
+    out_cache_loc: torch.Tensor        # int64 [T]: slot of token prefix + j
+    cu_q: torch.Tensor                 # int32 [B+1]
+    max_nodes: int
+
+
+def tree_prepare(page_table: torch.Tensor, page_table_ids: torch.Tensor, prefix_lens: torch.Tensor, parents: torch.Tensor,
+                 cu_q: torch.Tensor, page_size: int, max_nodes: int, new_pages: Optional[torch.Tensor] = None,
+                 new_page_off: Optional[torch.Tensor] = None) -> TreePlan:
+    """Metadata of a batch of draft trees, one launch (m355_tree_prepare): ancestor masks, positions and slots of all nodes, and
+    the page-table entries of new_pages (int32; request b owns new_pages[new_page_off[b]:new_page_off[b+1]], behind the pages of
+    its prefix).  parents int32 [T]: index of the parent inside the request, below the node's own, or -1."""
+    lib = _lib.load()
+    given = [("page_table", page_table), ("page_table_ids", page_table_ids), ("prefix_lens", prefix_lens), ("parents", parents),
+             ("cu_q", cu_q)]
+    if (new_pages is None) != (new_page_off is None):
+        raise _lib.MI355AttnError("tree_prepare: new_pages and new_page_off go together")
+    if new_pages is not None:
+        given += [("new_pages", new_pages), ("new_page_off", new_page_off)]
+    _device_of(given)
+    B, T = prefix_lens.numel(), parents.numel()
+    _vector("page_table_ids", page_table_ids, torch.int64, B), _vector("prefix_lens", prefix_lens, torch.int64, B)
+    _vector("parents", parents, torch.int32, T), _vector("cu_q", cu_q, torch.int32, B + 1)
+    if new_pages is not None:
+        _vector("new_pages", new_pages, torch.int32, new_pages.numel()), _vector("new_page_off", new_page_off, torch.int32, B + 1)
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 or page_size < 1:
+        raise _lib.MI355AttnError("tree_prepare: page_table must be int32 [rows, pages] with inner stride 1, page_size >= 1")
+    if not 1 <= max_nodes <= _lib.TREE_MAX_NODES:
+        raise _lib.MI355AttnError(f"tree_prepare: trees of 1 to {_lib.TREE_MAX_NODES} nodes are supported, got max_nodes {max_nodes}")
+    words = -(-max_nodes // 32)
+    dev = parents.device
+    mask = torch.empty((T, words), dtype=torch.int32, device=dev)
+    two = torch.empty((2, T), dtype=torch.int64, device=dev)
+    # (an empty new_pages has no address: the table is complete then)
+    fresh = new_pages is not None and new_pages.numel() > 0
+    check(lib.m355_tree_prepare(page_table.data_ptr(), _stride0(page_table, page_table.shape[1]), page_table.shape[0], page_table.shape[1],
+                                page_table_ids.data_ptr(), prefix_lens.data_ptr(), parents.data_ptr(), cu_q.data_ptr(),
+                                new_pages.data_ptr() if fresh else None, new_page_off.data_ptr() if fresh else None, B, T, max_nodes,
+                                page_size, mask.data_ptr(), words, two[0].data_ptr(), two[1].data_ptr(), current_stream()), "m355_tree_prepare")
+    return TreePlan(mask, two[0], two[1], cu_q, max_nodes)
+
+
+def tree_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
+              page_table_ids: torch.Tensor, prefix_lens: torch.Tensor, plan: TreePlan, page_size: int, num_heads: int,
+              max_seq_len: int, *, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+              workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of drafted nodes over the cached prefix and their ancestors (m355_tree_attn), after the nodes' K/V have been
+    written to plan.out_cache_loc.  max_seq_len >= the longest prefix + nodes; softcap / slopes as scored_attn, distances between
+    nodes being differences of depth."""
+    lib = _lib.load()
+    given = [("q", q), ("k_pool", k_pool), ("v_pool", v_pool), ("page_table", page_table), ("page_table_ids", page_table_ids),
+             ("prefix_lens", prefix_lens), ("mask", plan.mask), ("positions", plan.positions), ("cu_q", plan.cu_q)]
+    given += [(n, t) for n, t in (("slopes", slopes), ("workspace", workspace), ("out", out)) if t is not None]
+    _device_of(given)
+    B, T = prefix_lens.numel(), q.shape[0]
+    _vector("page_table_ids", page_table_ids, torch.int64, B), _vector("prefix_lens", prefix_lens, torch.int64, B)
+    _vector("plan.cu_q", plan.cu_q, torch.int32, B + 1), _vector("plan.positions", plan.positions, torch.int64, T)
+    if plan.mask.dtype != torch.int32 or plan.mask.dim() != 2 or plan.mask.shape[0] != T or not plan.mask.is_contiguous():
+        raise _lib.MI355AttnError(f"tree_attn: the plan is for {plan.mask.shape[0]} nodes, q has {T} rows")
+    if slopes is not None:
+        _vector("slopes", slopes, torch.float32, num_heads)
+    D = k_pool.shape[-1]
+    need = scored_workspace_bytes(B, T, num_heads, k_pool.shape[1], D, plan.max_nodes, max_seq_len) if workspace is None else 0
+    q2, pitch, out, workspace = _scored_buffers("tree_attn", q, k_pool, v_pool, page_table, num_heads, page_size, out, workspace, need)
+    W = num_heads * D
+    check(lib.m355_tree_attn(q2.data_ptr(), _stride0(q2, W), k_pool.data_ptr(), v_pool.data_ptr(), pitch, k_pool.shape[0],
+                             page_table.data_ptr(), _stride0(page_table, page_table.shape[1]), page_table.shape[0], page_table.shape[1],
+                             page_table_ids.data_ptr(), prefix_lens.data_ptr(), plan.cu_q.data_ptr(), plan.mask.data_ptr(),
+                             plan.mask.shape[1], plan.positions.data_ptr(), out.data_ptr(), _stride0(out, W), B, T, plan.max_nodes,
+                             max_seq_len, num_heads, k_pool.shape[1], D, page_size, float(D) ** -0.5 if scale is None else scale,
+                             softcap, _ptr(slopes), _ptr(workspace),
+                             0 if workspace is None else workspace.numel() * workspace.element_size(), dtype_code(q.dtype),
+                             current_stream()), "m355_tree_attn")
+    return out
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: Optional[torch.Tensor]   # fp32, shaped as the given tokens
+    entropy: torch.Tensor              # fp32 [T]
+    top_logprobs: torch.Tensor         # fp32 [T, top_k], largest first
+    top_ids: torch.Tensor              # int64 [T, top_k]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top_k: int = 0, temperature: float = 1.0,
+                   workspace: Optional[torch.Tensor] = None) -> TokenLogprobs:
+    """Log probabilities of `tokens` (int64 [T] or [T, n]; None: none) under softmax(logits / temperature), the rows' entropies
+    and their top_k alternatives, ties to the lower id, in one pass over logits [T, V] (m355_token_logprobs)."""
+    lib = _lib.load()
+    _device_of([("logits", logits)] + [(n, t) for n, t in (("tokens", tokens), ("workspace", workspace)) if t is not None])
+    if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1):
+        raise _lib.MI355AttnError(f"token_logprobs: logits must be [T, V] with inner stride 1, got {tuple(logits.shape)}")
+    T, V = logits.shape
+    if V < 1 or not 0 <= top_k <= min(V, _lib.MAX_TOP_LOGPROBS):
+        raise _lib.MI355AttnError(f"token_logprobs: top_k {top_k} of a vocabulary of {V} (at most {_lib.MAX_TOP_LOGPROBS} are supported)")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise _lib.MI355AttnError(f"token_logprobs: temperature must be positive, got {temperature}")
+    given, lp = 0, None
+    if tokens is not None:
+        if tokens.dtype != torch.int64 or tokens.dim() not in (1, 2) or tokens.shape[0] != T:
+            raise _lib.MI355AttnError(f"token_logprobs: tokens must be int64 [{T}] or [{T}, n], got {tokens.dtype} {tuple(tokens.shape)}")
+        tokens = tokens.contiguous()
+        given = 1 if tokens.dim() == 1 else tokens.shape[1]
+        lp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
+    entropy = torch.empty(T, dtype=torch.float32, device=logits.device)
+    top = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
+    ids = torch.empty((T, top_k), dtype=torch.int64, device=logits.device)
+    if workspace is None:
+        need = int(lib.m355_token_logprobs_workspace_bytes(T, V, top_k))
+        workspace = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    check(lib.m355_token_logprobs(logits.data_ptr(), logits.stride(0) if T > 1 else max(V, logits.stride(0)), _ptr(tokens), given, T, V, top_k,
+                                  temperature, _ptr(lp), entropy.data_ptr(), top.data_ptr(), ids.data_ptr(), _ptr(workspace),
+                                  0 if workspace is None else workspace.numel() * workspace.element_size(), dtype_code(logits.dtype),
+                                  current_stream()), "m355_token_logprobs")
+    return TokenLogprobs(lp, entropy, top, ids)

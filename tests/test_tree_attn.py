@@ -1,0 +1,166 @@
+"""Draft trees on the GPU: metadata against whole-number rules, attention against the definition in 64 bits."""
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from oracle.scored_ref import ancestors_ref, attend_ref
+from test_scored_attn import BF, DEV, HF, Case, check, slopes_of
+
+pytestmark = pytest.mark.gpu
+
+
+def trees(seed, sizes, bad=False):
+    rng = random.Random(seed)
+    out = []
+    for n in sizes:
+        p = [rng.randint(max(-1, j - 8), j - 1) for j in range(n)]
+        if bad and n > 3:
+            p[2], p[3] = 2, 9999                                          # itself and a node that is not there: roots
+        out.append(p)
+    return out
+
+
+def prepare(c, parents, table=None, **kw):
+    from mi355_attn import ops
+    flat = torch.tensor([x for p in parents for x in p], dtype=torch.int32, device=DEV)
+    return ops.tree_prepare(c.table.to(DEV) if table is None else table, c.rows.to(DEV), torch.tensor(c.pre, dtype=torch.int64, device=DEV), flat,
+                            torch.tensor(c.cu, dtype=torch.int32, device=DEV), c.ps, max(c.ext), **kw)
+
+
+def attn(c, plan, **kw):
+    from mi355_attn import ops
+    return ops.tree_attn(c.q.reshape(c.T, -1).to(DEV), c.pool(c.k), c.pool(c.v), c.table.to(DEV), c.rows.to(DEV),
+                         torch.tensor(c.pre, dtype=torch.int64, device=DEV), plan, c.ps, c.Hq, max(c.len), **kw)
+
+
+def want(c, parents, softcap=0.0, slopes=None):
+    outs, tols = [], []
+    for b, par in enumerate(parents):
+        seen, depth = ancestors_ref(par)
+        P, a = c.pre[b], c.cu[b]
+        rows = []
+        for j in range(len(par)):
+            up = sorted(seen[j])
+            rows.append((list(range(P)) + [P + x for x in up], list(range(P)) + [P + depth[x] for x in up], P + depth[j]))
+        o, t = attend_ref(c.q[a:a + len(par)], c.k, c.v, c.slots[b], rows, c.dtype, c.D ** -0.5, softcap, slopes)
+        outs.append(o), tols.append(t)
+    return torch.cat(outs), torch.cat(tols)
+
+
+@pytest.mark.parametrize("ps", [1, 3, 16])
+@pytest.mark.parametrize("pages", [True, False], ids=["new-pages", "complete-table"])
+def test_tree_metadata(ps, pages):
+    pre, ext = [0, 1, 15, 16, 40, 7], [1, 33, 64, 5, 100, 0]
+    c = Case(1, BF, (2, 1, 64), ps, pre, ext)
+    parents = trees(2, ext, bad=True)
+    full = c.table.clone()
+    kw, table = {}, c.table.clone().to(DEV)
+    if pages:
+        fresh, off = [], [0]
+        for b in range(c.B):
+            first, last = -(-pre[b] // ps), -(-c.len[b] // ps)
+            fresh += full[c.rows[b], first:last].tolist()
+            off.append(len(fresh))
+            table[c.rows[b], first:last] = -7
+        kw = dict(new_pages=torch.tensor(fresh, dtype=torch.int32, device=DEV), new_page_off=torch.tensor(off, dtype=torch.int32, device=DEV))
+    plan = prepare(c, parents, table=table, **kw)
+    assert torch.equal(table.cpu(), full)
+    mask = plan.mask.cpu().numpy().astype(np.int64) & 0xFFFFFFFF
+    t = 0
+    for b, par in enumerate(parents):
+        seen, depth = ancestors_ref(par)
+        for j in range(len(par)):
+            assert {32 * w + x for w in range(mask.shape[1]) for x in range(32) if mask[t, w] >> x & 1} == seen[j]
+            assert int(plan.positions[t]) == pre[b] + depth[j]
+            assert int(plan.out_cache_loc[t]) == c.slots[b][pre[b] + j]
+            t += 1
+
+
+def test_tree_metadata_past_the_table():
+    """Nodes past the table's width get no slot, and no page is entered beyond it."""
+    from mi355_attn import _lib, ops
+    table = torch.full((2, 6), 5, dtype=torch.int32, device=DEV)
+    plan = ops.tree_prepare(table[:, :3], torch.tensor([1], device=DEV), torch.tensor([10], device=DEV), torch.arange(-1, 5, dtype=torch.int32, device=DEV),
+                            torch.tensor([0, 6], dtype=torch.int32, device=DEV), 4, 6, new_pages=torch.tensor([9], dtype=torch.int32, device=DEV),
+                            new_page_off=torch.tensor([0, 1], dtype=torch.int32, device=DEV))
+    assert plan.out_cache_loc.tolist() == [22, 23] + [_lib.NO_SLOT] * 4
+    assert bool((table == 5).all())
+
+
+def test_long_chain_and_largest_tree():
+    n = 1024
+    c = Case(3, BF, (1, 1, 64), 16, [5], [n])
+    plan = prepare(c, [list(range(-1, n - 1))])
+    assert torch.equal(plan.positions.cpu(), 5 + torch.arange(n))
+    got = attn(c, plan).view(n, 1, 64)
+    pick = [0, 1, 26, 27, 59, 500, 1023]                                   # a chain is a causal extend
+    rows = [(list(range(5 + j + 1)), list(range(5 + j + 1)), 5 + j) for j in pick]
+    check(got[pick], *attend_ref(c.q[pick], c.k, c.v, c.slots[0], rows, BF, 64 ** -0.5))
+
+
+@pytest.mark.parametrize("mod", [dict(), dict(softcap=30.0), dict(slopes=True), dict(slopes=True, softcap=8.0)], ids=lambda m: "-".join(m) or "plain")
+@pytest.mark.parametrize("dtype,heads,ps,pre,ext", [
+    (BF, (4, 2, 64), 16, [0, 33, 100, 16], [1, 9, 33, 64]),
+    (HF, (3, 1, 128), 1, [1, 31, 32, 63], [40, 2, 7, 5]),
+    (BF, (8, 1, 128), 16, [2000, 5], [64, 3]),
+    (HF, (2, 2, 64), 5, [700], [100]),
+    (BF, (32, 8, 128), 16, [640], [8]),
+])
+def test_tree_attention(dtype, heads, ps, pre, ext, mod):
+    c = Case(4, dtype, heads, ps, pre, ext)
+    parents = trees(5, ext)
+    kw = dict(mod)
+    if "slopes" in kw:
+        kw["slopes"] = slopes_of(c.Hq)
+    ref = want(c, parents, **kw)
+    if "slopes" in kw:
+        kw["slopes"] = kw["slopes"].to(DEV)
+    got = attn(c, prepare(c, parents), **kw)
+    check(got, *ref)
+    assert torch.equal(got, attn(c, prepare(c, parents), **kw))
+
+
+def test_siblings_do_not_leak():
+    """NaN and infinities in one branch: its nodes say so, every other node is as if it were not there."""
+    c = Case(6, BF, (4, 1, 64), 16, [50], [12])
+    parents = [[-1, 0, 0, 1, 2, 3, 4, 2, 7, 0, 9, 10]]
+    for x in (2, 7):                                                        # node 2's branch: 2, 4, 6, 7, 8
+        c.v[c.slots[0][50 + x], 0, 3] = float("nan")
+        c.v[c.slots[0][50 + x], 0, 9] = float("inf")
+        c.k[c.slots[0][50 + x], 0, 1] = float("nan") if x == 7 else 1.0
+    got = attn(c, prepare(c, parents)).view(12, 4, 64).double().cpu()
+    ref, tol = want(c, parents)
+    fine = torch.isfinite(ref)
+    assert torch.equal(torch.isfinite(got), fine)
+    assert bool(((got - ref).abs() <= tol)[fine].all())
+    clean = [0, 1, 3, 5, 9, 10, 11]
+    assert bool(fine[clean].all()) and not bool(fine[[2, 4, 6]].all())
+
+
+def test_forest_without_a_prefix_and_masks_that_leave_nothing():
+    from mi355_attn import ops
+    c = Case(8, BF, (2, 1, 64), 4, [0, 0], [5, 3])
+    parents = [[-1, -1, 0, 1, -1], [-1, 0, 1]]
+    plan = prepare(c, parents)
+    check(attn(c, plan), *want(c, parents))
+    none = plan._replace(mask=torch.zeros_like(plan.mask))
+    assert bool((attn(c, none) == 0).all())
+
+
+def test_refusals():
+    from mi355_attn import ops
+    from mi355_attn._lib import MI355AttnError
+    c = Case(9, BF, (2, 1, 64), 16, [5], [4])
+    plan = prepare(c, [[-1, 0, 1, 2]])
+    with pytest.raises(MI355AttnError, match="nodes"):
+        attn(c, plan._replace(mask=plan.mask[:3]))
+    with pytest.raises(MI355AttnError, match="positions"):
+        attn(c, plan._replace(positions=plan.positions[:3]))
+    with pytest.raises(MI355AttnError, match="1024"):
+        ops.tree_prepare(c.table.to(DEV), c.rows.to(DEV), torch.tensor([5], device=DEV), torch.zeros(4, dtype=torch.int32, device=DEV), plan.cu_q, 16, 2000)
+    with pytest.raises(MI355AttnError, match="go together"):
+        prepare(c, [[-1, 0, 1, 2]], new_pages=torch.zeros(1, dtype=torch.int32, device=DEV))
+    with pytest.raises(MI355AttnError, match="parents"):
+        ops.tree_prepare(c.table.to(DEV), c.rows.to(DEV), torch.tensor([5], device=DEV), torch.zeros(4, device=DEV), plan.cu_q, 16, 4)
