@@ -6,86 +6,741 @@
 //
 // visible: an interval (causal, window, document start, bidirectional prefix: scored_rules.h visible_range) or, for a tree of
 // drafted tokens, the prefix and the row's ancestors (tree_bits).
+//
+// A query row is a (token, q head of the group) pair, token-major, so the G heads that share a kv head share its loads.  Two
+// kernels, by the rows a request brings: scored_few_kernel (decode steps, small trees: HBM-bound) and scored_wide_kernel (long
+// extends, large trees: bound by the vector unit's exponentials and the matrix unit).  Both walk [lo_min, hi_max) of their
+// rows only, in one pass with the running maximum and sum of the softmax, and cut that range into splits when there are too few row
+// blocks for 256 CUs; scored_merge_kernel then joins the splits.  Nothing is accumulated by atomics: results do not depend on
+// an order of arrival.
+//
+// Masked keys.  A mask is one 32-bit word per (row, tile of 32 keys), whatever made it, and is looked at in tiles that some row
+// sees in part only.  Scores of masked keys become -inf, so what K holds there cannot matter; the weight 0 times an infinity
+// or NaN in V would be NaN, so in those tiles V is looked through and, where something is found, infinities and NaN are taken out
+// of the matrix product and added to the rows that do see the key.
+#include "prefill_common.h"
 #include "scored_common.h"
+#include "stream_plan.h"
 
 namespace m355 {
 
-// One wave per (query row, q head): lanes are keys in the score product and head-dim elements in the value sum.  Simple and
-// right for every shape; each K/V row is read again by every row and head that sees it.
-template <int D, bool F16>
-__global__ __launch_bounds__(64) void scored_rows_kernel(const ScoredParams p) {
-    __shared__ float qs[D], ps[64];
-    __shared__ int32_t ss[64];
-    const int lane = threadIdx.x, j = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+// softmax(-inf everywhere so far): the difference of two -inf would be NaN
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+
+// ------------------------------------------------------------------------------------------------------------------------
+// Few rows: a workgroup takes up to 16 RT rows of one (request, kv head) and one split of the keys.  Its four waves walk tiles
+// of 32 keys on their own (tile 4 i + wave), each with its own two-stage LDS ring filled by LDS-DMA, and hold all rows: K and V
+// are read from memory once per workgroup and from LDS once per wave, and no barrier sits in the loop.  The waves' results
+// meet in LDS at the end.
+//   S^T[key, row]  = K[32 x D] . Q^T[D x 16]   v_mfma_f32_16x16x32: a lane owns one row and 8 of the tile's keys
+//   O^T[d, row]   += V^T[D x 32] . P^T[32 x 16]   P^T is the S^T accumulator rounded in place, V^T is read transposed
+// ------------------------------------------------------------------------------------------------------------------------
+constexpr int kFewSlots = 2048;                       // tokens whose pool slots are in LDS at a time
+
+template <int D, int RT, bool MOD, bool F16>
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void scored_few_kernel(const ScoredParams p) {
+    using M = MG<D>;
+    constexpr int RW = 16 * RT, PITCH = D + 4;
+    constexpr int RING = 8 * M::STAGEB, JOIN = 4 * RW * (PITCH + 2) * 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[RING > JOIN ? RING : JOIN];
+    __shared__ int32_t slots[kFewSlots];
+    const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+
+    // ---- which rows and keys.  Row blocks of one (request, kv head, split) follow one another on one XCD (workgroups go round
+    // the 8 XCDs), so that they share the keys in its L2; the kv head rotates with the unit so that no XCD reads one column only.
+    const int y = blockIdx.x >> 3, rb = y % p.blocks;
+    const int u = (y / p.blocks) * 8 + (blockIdx.x & 7);
+    if (u >= p.splits * p.B * p.Hkv) return;
+    const int h = (u + u / p.Hkv) % p.Hkv, b = u / p.Hkv % p.B, sp = u / (p.Hkv * p.B);
     const ReqSpan r = load_span(p, b);
-    if (j >= r.E) return;
-    const int64_t t = r.q0 + j;
+    const int row0 = rb * RW, rows = r.E * p.G;
+    if (row0 >= rows) return;
     const int32_t* pt_row = table_row(p, b);
-    const bool tree = p.mask != nullptr;
-    int32_t pos = r.P + j;
-    KeyRange v;
-    if (tree) {
-        v = {0, r.L};
-        if (p.slopes) pos = (int32_t)p.positions[t];
-    } else {
-        v = visible_range(pos, r.L, p.window, p.doc_starts ? p.doc_starts[t] : 0, p.bidir ? p.bidir[b] : 0);
+
+    // ---- the lane's rows
+    int32_t lo[RT], hi[RT], pos[RT], tr[RT], gr[RT];
+    bool ok[RT];
+    float slope[RT];
+    BlockRange br = block_range(p, r, b, row0 / p.G, imin(r.E - 1, (row0 + RW - 1) / p.G));
+    if (p.doc_starts) br = {0x7fffffff, 0, 0, 0x7fffffff};
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+        const int m = row0 + 16 * x + n;
+        ok[x] = m < rows;
+        const int j = ok[x] ? m / p.G : 0;
+        gr[x] = ok[x] ? m - j * p.G : 0;
+        tr[x] = r.q0 + j;
+        pos[x] = r.P + j;
+        if (p.mask) {
+            lo[x] = 0; hi[x] = r.L;
+            if (MOD && p.slopes) pos[x] = (int32_t)p.positions[tr[x]];
+        } else {
+            const KeyRange v = visible_range(pos[x], r.L, p.window, p.doc_starts ? p.doc_starts[tr[x]] : 0, p.bidir ? p.bidir[b] : 0);
+            lo[x] = v.lo; hi[x] = v.hi;
+        }
+        slope[x] = MOD && p.slopes ? p.slopes[h * p.G + gr[x]] * kLog2e : 0.f;
+        if (p.doc_starts && ok[x]) {
+            if (lo[x] < hi[x]) { br.lo_min = imin(br.lo_min, lo[x]); br.hi_max = imax(br.hi_max, hi[x]); }
+            br.lo_max = imax(br.lo_max, lo[x]); br.hi_min = imin(br.hi_min, hi[x]);
+        }
     }
-    for (int d = lane; d < D; d += 64) {
-        const uint32_t w = p.q[t * p.q_stride + (int64_t)h * D + d];
-        qs[d] = unpack16_lo<F16>(w);
+    if (p.doc_starts) {
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) {
+            br.lo_min = imin(br.lo_min, __shfl_xor(br.lo_min, x)); br.hi_max = imax(br.hi_max, __shfl_xor(br.hi_max, x));
+            br.lo_max = imax(br.lo_max, __shfl_xor(br.lo_max, x)); br.hi_min = imin(br.hi_min, __shfl_xor(br.hi_min, x));
+        }
+    }
+    const int lo_min = __builtin_amdgcn_readfirstlane(br.lo_min), hi_max = __builtin_amdgcn_readfirstlane(br.hi_max);
+    const int lo_max = __builtin_amdgcn_readfirstlane(br.lo_max), hi_min = __builtin_amdgcn_readfirstlane(br.hi_min);
+    const int first = lo_min & ~31, keys = lo_min < hi_max ? hi_max - first : 0;
+    const int active = imax(1, imin(p.splits, (keys + p.chunk - 1) / p.chunk));
+    if (sp >= active) return;
+    const int t0 = first + sp * p.chunk, t1 = keys ? (sp == active - 1 ? hi_max : t0 + p.chunk) : t0;
+
+    bf16x8 qf[RT][M::KS];
+#pragma unroll
+    for (int x = 0; x < RT; ++x)
+#pragma unroll
+        for (int s = 0; s < M::KS; ++s) {
+            u32x4 w = {0u, 0u, 0u, 0u};
+            if (ok[x]) w = *reinterpret_cast<const u32x4*>(p.q + tr[x] * p.q_stride + (int64_t)(h * p.G + gr[x]) * D + 32 * s + 8 * kg);
+            qf[x][s] = __builtin_bit_cast(bf16x8, w);
+        }
+
+    f32x4 O[RT][M::DT];
+    float m_run[RT], l_run[RT];
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+        m_run[x] = -INFINITY; l_run[x] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < M::DT; ++dt) O[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // ---- per-lane constants of the DMA and of the LDS reads (stream_plan.h MG: chunk ch of a row sits at ch ^ s(row))
+    const int drow = lane / M::C, dch = lane % M::C;
+    uint8_t* const ring = smem + wid * 2 * M::STAGEB;
+    const uint32_t ring0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
+    const uint8_t* kbase = reinterpret_cast<const uint8_t*>(p.k_pool) + (int64_t)h * M::ROWB;
+    const uint8_t* vbase = reinterpret_cast<const uint8_t*>(p.v_pool) + (int64_t)h * M::ROWB;
+    const uint64_t row_bytes = (uint64_t)p.row_elems * 2;
+    int koff[M::NI], voff[M::NI];
+#pragma unroll
+    for (int i = 0; i < M::NI; ++i) {
+        koff[i] = 16 * (dch ^ M::sK(i * M::RPI + drow));
+        voff[i] = 16 * (dch ^ M::sV(i * M::RPI + drow));
+    }
+    const int ka0 = n * M::ROWB + 16 * (kg ^ M::sK(n));
+    const int vrow = 4 * kg + (n >> 2);
+    const int va0 = vrow * M::ROWB + 16 * (M::sV(vrow) | ((n & 3) >> 1)) + 8 * (n & 1);
+
+    int w0 = t0, wn = 0;                              // the slot window: tokens w0 .. w0 + wn
+    auto issue = [&](const int tile, const int st) {
+        int64_t ro[M::NI];
+#pragma unroll
+        for (int i = 0; i < M::NI; ++i) ro[i] = slots[imin(32 * tile + i * M::RPI + drow, wn - 1)];
+#pragma unroll
+        for (int i = 0; i < M::NI; ++i) {
+            glds16p<1>(kbase + ro[i] * row_bytes + koff[i], ring0 + st * M::STAGEB + 1024 * i);
+            glds16p<1>(vbase + ro[i] * row_bytes + voff[i], ring0 + st * M::STAGEB + M::TILEB + 1024 * i);
+        }
+    };
+    auto v_frag = [&](const uint8_t* st, const int dt) {
+        const uint8_t* va = st + M::TILEB + (va0 ^ (32 * dt));
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(uintptr_t)(uint32_t)(uintptr_t)va);
+        const s16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(uintptr_t)(uint32_t)(uintptr_t)(va + 16 * M::ROWB));
+        return __builtin_bit_cast(bf16x8, s16x8{a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]});
+    };
+    auto consume = [&](const int base, const int stage) {
+        const uint8_t* st = ring + stage * M::STAGEB;
+        f32x4 s0[RT], s1[RT];
+#pragma unroll
+        for (int x = 0; x < RT; ++x) s0[x] = s1[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < M::KS; ++s) {
+            const bf16x8 a0 = *reinterpret_cast<const bf16x8*>(st + (ka0 ^ (64 * s)));
+            const bf16x8 a1 = *reinterpret_cast<const bf16x8*>(st + 16 * M::ROWB + (ka0 ^ (64 * s)));
+#pragma unroll
+            for (int x = 0; x < RT; ++x) {
+                s0[x] = mfma_16x16x32<F16>(a0, qf[x][s], s0[x]);
+                s1[x] = mfma_16x16x32<F16>(a1, qf[x][s], s1[x]);
+            }
+        }
+        // this lane: row n of each tile, keys base + 4 kg + i and base + 16 + 4 kg + i
+        if constexpr (MOD) {
+            if (p.cap_log2 > 0.f) {
+#pragma unroll
+                for (int x = 0; x < RT; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { s0[x][i] = cap_score(p, s0[x][i]); s1[x][i] = cap_score(p, s1[x][i]); }
+            } else {
+#pragma unroll
+                for (int x = 0; x < RT; ++x) { s0[x] *= p.scale_log2; s1[x] *= p.scale_log2; }
+            }
+            if (p.slopes) {
+                if (p.mask && base + 32 > r.P) {          // some keys are nodes: their positions are their depths
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int tok = base + 16 * (i >> 2) + 4 * kg + (i & 3);
+                        const int node = imin(imax(tok - r.P, 0), r.E - 1);
+                        const int kp = tok < r.P ? tok : (int)p.positions[r.q0 + node];
+#pragma unroll
+                        for (int x = 0; x < RT; ++x) {
+                            const float away = fabsf((float)(pos[x] - kp));
+                            if (i < 4) s0[x][i & 3] = fmaf(-slope[x], away, s0[x][i & 3]);
+                            else s1[x][i & 3] = fmaf(-slope[x], away, s1[x][i & 3]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < RT; ++x) {
+                        const float d = (float)(pos[x] - base - 4 * kg);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            s0[x][i] = fmaf(-slope[x], fabsf(d - (float)i), s0[x][i]);
+                            s1[x][i] = fmaf(-slope[x], fabsf(d - (float)(16 + i)), s1[x][i]);
+                        }
+                    }
+                }
+            }
+        }
+        const bool part = base < lo_max || base + 32 > hi_min;             // wave-uniform
+        uint32_t bits[RT];
+        bool bad = false;
+        if (part) {
+#pragma unroll
+            for (int x = 0; x < RT; ++x) {
+                bits[x] = row_bits(p, r, tr[x], lo[x], hi[x], base);
+                const uint32_t w = bits[x] >> (4 * kg);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s0[x][i] = (w >> i) & 1u ? s0[x][i] : -INFINITY;
+                    s1[x][i] = (w >> (16 + i)) & 1u ? s1[x][i] : -INFINITY;
+                }
+            }
+            bool any = false;
+#pragma unroll
+            for (int dt = 0; dt < M::DT; ++dt) any = any || frag_nonfinite<F16>(v_frag(st, dt));
+            bad = __any(any);
+        }
+        bf16x8 pf[RT];
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+            float mx = fmaxf(fmaxf(fmaxf(s0[x][0], s0[x][1]), fmaxf(s0[x][2], s0[x][3])), fmaxf(fmaxf(s1[x][0], s1[x][1]), fmaxf(s1[x][2], s1[x][3])));
+            float a, c;
+            lane_pair<16>(mx, a, c);
+            mx = fmaxf(a, c);
+            lane_pair<32>(mx, a, c);
+            mx = fmaxf(a, c);
+            if constexpr (!MOD) mx *= p.scale_log2;
+            // the running maximum moves only when beaten by 2^kLazyMax: rescaling is rare, weights stay below 2^kLazyMax
+            const float m_new = mx > m_run[x] + kLazyMax ? mx : m_run[x];
+            const float alpha = m_new == m_run[x] ? 1.f : exp2_fast(m_run[x] - m_new);
+            m_run[x] = m_new;
+            const float mu = finite_max(m_new);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s0[x][i] = exp2_fast(MOD ? s0[x][i] - mu : fmaf(s0[x][i], p.scale_log2, -mu));
+                s1[x][i] = exp2_fast(MOD ? s1[x][i] - mu : fmaf(s1[x][i], p.scale_log2, -mu));
+                sum += s0[x][i] + s1[x][i];
+            }
+            l_run[x] = fmaf(l_run[x], alpha, sum);
+            if (__any(alpha != 1.f)) {
+#pragma unroll
+                for (int dt = 0; dt < M::DT; ++dt) O[x][dt] *= alpha;
+            }
+            pf[x] = __builtin_bit_cast(bf16x8, u32x4{pack16<F16>(s0[x][0], s0[x][1]), pack16<F16>(s0[x][2], s0[x][3]),
+                                                     pack16<F16>(s1[x][0], s1[x][1]), pack16<F16>(s1[x][2], s1[x][3])});
+        }
+#pragma unroll
+        for (int dt = 0; dt < M::DT; ++dt) {
+            bf16x8 av = v_frag(st, dt);
+            if (bad) av = frag_finite<F16>(av);
+#pragma unroll
+            for (int x = 0; x < RT; ++x) O[x][dt] = mfma_16x16x32<F16>(av, pf[x], O[x][dt]);
+        }
+        if (bad) {                                                         // rare: infinities and NaN, for the rows that see them
+            for (int tk = 0; tk < 32; ++tk) {
+                const uint8_t* vr = st + M::TILEB + tk * M::ROWB + 8 * (kg & 1);
+#pragma unroll
+                for (int dt = 0; dt < M::DT; ++dt) {
+                    const f32x4 e = nonfinite4<F16>(*reinterpret_cast<const uint2*>(vr + 16 * ((2 * dt + (kg >> 1)) ^ M::sV(tk))));
+#pragma unroll
+                    for (int x = 0; x < RT; ++x)
+                        if ((bits[x] >> tk) & 1u) O[x][dt] += e;
+                }
+            }
+        }
+    };
+
+    for (; w0 < t1; w0 += kFewSlots) {
+        wn = imin(kFewSlots, t1 - w0);
+        __syncthreads();
+        for (int i = threadIdx.x; i < wn; i += 256) slots[i] = slot_of(p, pt_row, w0 + i);
+        __syncthreads();
+        const int nt = (wn + 31) >> 5;
+        if (wid < nt) issue(wid, 0);
+        for (int t = wid; t < nt; t += 8) {
+            if (t + 4 < nt) { issue(t + 4, 1); wait_vmcnt<2 * M::NI>(); } else wait_vmcnt<0>();
+            consume(w0 + 32 * t, 0);
+            if (t + 4 >= nt) break;
+            if (t + 8 < nt) { issue(t + 8, 0); wait_vmcnt<2 * M::NI>(); } else wait_vmcnt<0>();
+            consume(w0 + 32 * (t + 4), 1);
+        }
+    }
+
+    // ---- the four waves' results meet in LDS
+    float* const jo = reinterpret_cast<float*>(smem);
+    float* const jm = jo + 4 * RW * PITCH;                                  // (m, l) per wave and row
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+        float a, c;
+        lane_pair<16>(l_run[x], a, c);
+        float l = a + c;
+        lane_pair<32>(l, a, c);
+        l = a + c;
+        const int row = wid * RW + 16 * x + n;
+        if (kg == 0) *reinterpret_cast<float2*>(jm + 2 * row) = make_float2(m_run[x], l);
+#pragma unroll
+        for (int dt = 0; dt < M::DT; ++dt) *reinterpret_cast<f32x4*>(jo + row * PITCH + 16 * dt + 4 * kg) = O[x][dt];
     }
     __syncthreads();
-    const float slope = p.slopes ? p.slopes[h] : 0.f;
-    const int64_t hoff = (int64_t)(h / p.G) * D;
-    float m = -INFINITY, l = 0.f, o[D / 64];
-    for (int x = 0; x < D / 64; ++x) o[x] = 0.f;
-    for (int base = v.lo & ~31; base < v.hi; base += 64) {
-        const int tok = base + lane;
-        const int half = base + (lane & 32);
-        const uint32_t bits = tree ? tree_bits(p.mask + t * p.words, p.words, r.P, v.hi, half) : range_bits(v.lo, v.hi, half);
-        const bool seen = (bits >> (lane & 31)) & 1u;
-        float s = -INFINITY;
-        int32_t slot = 0;
-        if (seen) {
-            slot = slot_of(p, pt_row, tok);
-            const uint16_t* kr = p.k_pool + (int64_t)slot * p.row_elems + hoff;
-            float acc = 0.f;
-            for (int c = 0; c < D / 8; ++c) {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(kr + 8 * c);
-                for (int y = 0; y < 4; ++y) acc += unpack16_lo<F16>(w[y]) * qs[8 * c + 2 * y] + unpack16_hi<F16>(w[y]) * qs[8 * c + 2 * y + 1];
-            }
-            s = acc * p.scale;
-            if (p.cap > 0.f) s = p.cap * tanhf(s / p.cap);
-            if (p.slopes) {
-                const int32_t kp = tree && tok >= r.P ? (int32_t)p.positions[r.q0 + tok - r.P] : tok;
-                s -= slope * fabsf((float)(pos - kp));
-            }
+    constexpr int CH = D / 4;
+    for (int i = threadIdx.x; i < RW * CH; i += 256) {
+        const int row = i / CH, c = i % CH, m = row0 + row;
+        if (m >= rows) break;
+        float mw[4], mx = -INFINITY, l = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) { mw[w] = jm[2 * (w * RW + row)]; mx = fmaxf(mx, mw[w]); }
+        const float mu = finite_max(mx);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float e = exp2_fast(mw[w] - mu);
+            l = fmaf(e, jm[2 * (w * RW + row) + 1], l);
+            o += *reinterpret_cast<const f32x4*>(jo + (w * RW + row) * PITCH + 4 * c) * e;
         }
-        float mt = s;
-        for (int x = 32; x; x >>= 1) mt = fmaxf(mt, __shfl_xor(mt, x));
-        const float mn = fmaxf(m, mt);
-        const float mu = mn == -INFINITY ? 0.f : mn;
-        const float alpha = exp2_fast((m - mu) * kLog2e);
-        float e = exp2_fast((s - mu) * kLog2e);
-        m = mn;
-        ps[lane] = e;
-        ss[lane] = seen ? slot : -1;
-        for (int x = 32; x; x >>= 1) e += __shfl_xor(e, x);
-        l = l * alpha + e;
-        __syncthreads();
-        for (int x = 0; x < D / 64; ++x) o[x] *= alpha;
-        for (int k = 0; k < 64; ++k) {
-            if (ss[k] < 0) continue;
-            const uint16_t* vr = p.v_pool + (int64_t)ss[k] * p.row_elems + hoff;
-            for (int x = 0; x < D / 64; ++x) o[x] += ps[k] * unpack16_lo<F16>((uint32_t)vr[lane + 64 * x]);
+        const int j = m / p.G, head = h * p.G + m - j * p.G;
+        const int64_t item = (int64_t)(r.q0 + j) * p.Hq + head;
+        if (active > 1) {
+            float* wo = p.part + (item * p.splits + sp) * (D + 4);
+            *reinterpret_cast<f32x4*>(wo + 4 * c) = o;
+            if (c == 0) *reinterpret_cast<float2*>(wo + D) = make_float2(mx, l);
+        } else {
+            const float inv = 1.f / l;
+            uint2 w = {0u, 0u};
+            if (l != 0.f) w = make_uint2(pack16<F16>(o[0] * inv, o[1] * inv), pack16<F16>(o[2] * inv, o[3] * inv));
+            *reinterpret_cast<uint2*>(p.out + (int64_t)(r.q0 + j) * p.o_stride + (int64_t)head * D + 4 * c) = w;
         }
-        __syncthreads();
+        if (sp == 0 && c == 0 && p.splits > 1) p.part_n[item] = active;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    for (int x = 0; x < D / 64; ++x)
-        p.out[t * p.o_stride + (int64_t)h * D + lane + 64 * x] = (uint16_t)(pack16<F16>(l == 0.f ? 0.f : o[x] * inv, 0.f) & 0xffffu);
 }
 
+// ------------------------------------------------------------------------------------------------------------------------
+// Many rows: the four waves of a workgroup own 32 consecutive rows each of one (request, kv head) and walk the keys together, a
+// pair of 32-key tiles at a time, brought into LDS once per workgroup by LDS-DMA (two pairs deep).  The matrix products are
+// those of prefill_attn.hip (v_mfma_f32_32x32x16, a lane owns one row and 16 of a tile's keys); what differs is the score
+// stage between them and the range that is walked.
+// ------------------------------------------------------------------------------------------------------------------------
+template <int D, bool MOD, bool F16>
+__global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams p) {
+    using W = WgCfg<D>;
+    constexpr int NW = 4, NBUF = 4, ROWS = 32 * NW, IPW = 2 * W::NI / NW, HP = IPW / 2;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[NBUF * W::BUFB];      // NBUF K tiles, NBUF V tiles
+    __shared__ int32_t slotw[kSlotWin];
+    __shared__ int32_t wlim[NW][2];
+    const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int l = threadIdx.x & 63, c = l & 31, hh = l >> 5;
+
+    // ---- which rows: all row blocks of one (request, kv head), which walk much the same keys, on one XCD, the last (longest
+    // under a causal mask) first; pairs left over after the full rounds of 8 are spread over all XCDs
+    const int n_bh = p.B * p.Hkv, mapped = (n_bh >> 3) * 8 * p.blocks;
+    int tb, bh;
+    if ((int)blockIdx.x < mapped) {
+        const int item = blockIdx.x >> 3;
+        tb = p.blocks - 1 - item % p.blocks; bh = (item / p.blocks) * 8 + (blockIdx.x & 7);
+    } else {
+        const int item = blockIdx.x - mapped;
+        tb = p.blocks - 1 - item % p.blocks; bh = (n_bh & ~7) + item / p.blocks;
+    }
+    const int h = bh % p.Hkv, b = bh / p.Hkv, sp = blockIdx.y;
+    const ReqSpan r = load_span(p, b);
+    const int rows = r.E * p.G;
+    if (ROWS * tb >= rows) return;                                 // whole workgroup: no barrier has been reached yet
+    const int32_t* pt_row = table_row(p, b);
+
+    // ---- this lane's row and the limits of its wave and workgroup
+    const int row0 = ROWS * tb + 32 * wid, mrow = row0 + c;
+    const bool valid = mrow < rows;
+    const int j = valid ? mrow / p.G : 0, g = valid ? mrow - j * p.G : 0;
+    const int64_t t = r.q0 + j;
+    int32_t pos = r.P + j, lo = 0, hi = r.L;
+    BlockRange br = {0x7fffffff, 0, 0, 0x7fffffff};                // the wave's rows
+    if (p.mask) {
+        if (MOD && p.slopes) pos = (int32_t)p.positions[t];
+    } else {
+        const KeyRange v = visible_range(pos, r.L, p.window, p.doc_starts ? p.doc_starts[t] : 0, p.bidir ? p.bidir[b] : 0);
+        lo = v.lo; hi = v.hi;
+    }
+    if (!p.doc_starts) {
+        if (row0 < rows) br = block_range(p, r, b, row0 / p.G, imin(r.E - 1, (row0 + 31) / p.G));
+    } else {
+        if (valid) {
+            if (lo < hi) { br.lo_min = lo; br.hi_max = hi; }
+            br.lo_max = lo; br.hi_min = hi;
+        }
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            br.lo_min = imin(br.lo_min, __shfl_xor(br.lo_min, x)); br.hi_max = imax(br.hi_max, __shfl_xor(br.hi_max, x));
+            br.lo_max = imax(br.lo_max, __shfl_xor(br.lo_max, x)); br.hi_min = imin(br.hi_min, __shfl_xor(br.hi_min, x));
+        }
+    }
+    if (br.lo_min >= br.hi_max) { br.lo_min = 0x7fffffff; br.hi_max = 0; }
+    if (l == 0) { wlim[wid][0] = br.lo_min; wlim[wid][1] = br.hi_max; }
+    const int w_lo_min = __builtin_amdgcn_readfirstlane(br.lo_min), w_hi_max = __builtin_amdgcn_readfirstlane(br.hi_max);
+    const int w_lo_max = __builtin_amdgcn_readfirstlane(br.lo_max), w_hi_min = __builtin_amdgcn_readfirstlane(br.hi_min);
+
+    bf16x8 qf[W::KS];
+    f32x16 o[W::DT];
+    {
+        const uint16_t* qp = p.q + t * p.q_stride + (int64_t)(h * p.G + g) * D + hh * 8;
+#pragma unroll
+        for (int s = 0; s < W::KS; ++s) {
+            u32x4 v = u32x4{0u, 0u, 0u, 0u};
+            if (valid) v = *reinterpret_cast<const u32x4*>(qp + s * 16);
+            qf[s] = __builtin_bit_cast(bf16x8, v);
+        }
+#pragma unroll
+        for (int dt = 0; dt < W::DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+    }
+    const float slope = MOD && p.slopes ? p.slopes[h * p.G + g] * kLog2e : 0.f;
+    __syncthreads();
+    int lo_wg = wlim[0][0], hi_wg = wlim[0][1];
+#pragma unroll
+    for (int x = 1; x < NW; ++x) { lo_wg = imin(lo_wg, wlim[x][0]); hi_wg = imax(hi_wg, wlim[x][1]); }
+    lo_wg = __builtin_amdgcn_readfirstlane(lo_wg); hi_wg = __builtin_amdgcn_readfirstlane(hi_wg);
+    const bool none = lo_wg >= hi_wg;
+    const int pair0 = none ? 0 : lo_wg >> 6, pairs_end = none ? 0 : (hi_wg + 63) >> 6, n_tiles = (hi_wg + 31) >> 5;
+    const int per = p.chunk >> 6;
+    const int active = imax(1, imin(p.splits, (pairs_end - pair0 + per - 1) / per));
+    if (sp >= active) return;
+    const int p_begin = pair0 + sp * per, n_pairs = sp == active - 1 ? pairs_end : p_begin + per;   // exclusive end
+
+    // ---- DMA duty of this wave (see prefill_attn.hip): pieces of 1 KiB of the pair's K and V tiles
+    const int drow = l / W::C, dch = l % W::C;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
+    const uint8_t* kbase = reinterpret_cast<const uint8_t*>(p.k_pool) + (int64_t)h * W::ROWB;
+    const uint8_t* vbase = reinterpret_cast<const uint8_t*>(p.v_pool) + (int64_t)h * W::ROWB;
+    const uint64_t row_bytes = (uint64_t)p.row_elems * 2;
+    int cur_win = -1;
+    auto fill_slots = [&](int win) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSlotWin / 256; ++k) {
+            const int i = (int)threadIdx.x + 256 * k;
+            slotw[i] = slot_of(p, pt_row, imin(win * kSlotWin + i, hi_wg - 1));
+        }
+        __syncthreads();
+        cur_win = win;
+    };
+    // a pair past the end fetches the last one again (masked, into a vacated buffer): every pair costs every wave the same
+    // number of DMA instructions and the counted waits are static
+    auto pair_slots = [&](int pair, int32_t (&sl)[IPW]) {
+        pair = pair < n_pairs ? pair : n_pairs - 1;
+        if ((2 * pair) / (kSlotWin / 32) != cur_win) fill_slots((2 * pair) / (kSlotWin / 32));   // workgroup-uniform
+#pragma unroll
+        for (int x = 0; x < IPW; ++x) {
+            const int tile = 2 * pair + x / HP < n_tiles ? 2 * pair + x / HP : n_tiles - 1;
+            sl[x] = slotw[((tile * 32) & (kSlotWin - 1)) + (wid + NW * (x % HP)) * W::RPI + drow];
+        }
+    };
+    uint32_t kch[HP], vch[HP];
+#pragma unroll
+    for (int y = 0; y < HP; ++y) {
+        const int row = (wid + NW * y) * W::RPI + drow;
+        kch[y] = 16 * (dch ^ W::sK(row));
+        vch[y] = 16 * (dch ^ W::sV(row));
+    }
+    auto piece = [&](const bool is_v, const int x, const int32_t slot, const int buf0) {
+        const uint64_t off = (uint64_t)(uint32_t)slot * row_bytes + (is_v ? vch[x % HP] : kch[x % HP]);
+        glds16p<M355_PREFILL_POLICY>((is_v ? vbase : kbase) + off,
+               lds0 + (is_v ? NBUF * W::TILEB : 0) + (buf0 + x / HP) * W::TILEB + 1024 * (wid + NW * (x % HP)));
+    };
+
+    uint32_t kaddr[W::KS], vaddr[W::DT];
+    {
+        const int ksw = W::sK(c);
+#pragma unroll
+        for (int s = 0; s < W::KS; ++s) kaddr[s] = lds0 + c * W::ROWB + 16 * ((2 * s + hh) ^ ksw);
+        const int gidx = l >> 4, li = l & 15;
+        const int vr = 4 * hh + (li >> 2), vcol = 2 * (gidx & 1) + ((li & 3) >> 1);
+#pragma unroll
+        for (int dt = 0; dt < W::DT; ++dt)
+            vaddr[dt] = lds0 + NBUF * W::TILEB + vr * W::ROWB + 16 * ((4 * dt + vcol) ^ W::sV(vr)) + 8 * (li & 1);
+    }
+    auto rdk = [&](const int buf, const int s) {
+        return *reinterpret_cast<const bf16x8 __attribute__((address_space(3)))*>((uintptr_t)(kaddr[s] + buf * W::TILEB));
+    };
+    auto rdv = [&](const int buf, const int f) {
+        const uint32_t a0 = vaddr[f >> 1] + buf * W::TILEB + 16 * (f & 1) * W::ROWB;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(uintptr_t)a0);
+        const s16x4 e = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(uintptr_t)(a0 + 8 * W::ROWB));
+        return __builtin_bit_cast(bf16x8, s16x8{a[0], a[1], a[2], a[3], e[0], e[1], e[2], e[3]});
+    };
+    // lane: keys base + (i & 3) + 8 (i >> 2) + 4 hh
+    auto modify = [&](f32x16& s, const int base) {
+        if (p.cap_log2 > 0.f) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = cap_score(p, s[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] *= p.scale_log2;
+        }
+        if (p.slopes) {
+            if (p.mask && base + 32 > r.P) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int tok = base + (i & 3) + 8 * (i >> 2) + 4 * hh;
+                    const int node = imin(imax(tok - r.P, 0), r.E - 1);
+                    const int kp = tok < r.P ? tok : (int)p.positions[r.q0 + node];
+                    s[i] = fmaf(-slope, fabsf((float)(pos - kp)), s[i]);
+                }
+            } else {
+                const float d = (float)(pos - base - 4 * hh);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = fmaf(-slope, fabsf(d - (float)((i & 3) + 8 * (i >> 2))), s[i]);
+            }
+        }
+    };
+    auto mask = [&](f32x16& s, const uint32_t bits) {
+        const uint32_t w = bits >> (4 * hh);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = (w >> ((i & 3) + 8 * (i >> 2))) & 1u ? s[i] : -INFINITY;
+    };
+    float m_run = -INFINITY, l_run = 0.f;
+    auto new_max = [&](float mx) {
+        float a, e;
+        lane_pair<32>(mx, a, e);
+        mx = fmaxf(a, e);
+        if constexpr (!MOD) mx *= p.scale_log2;
+        const float m_new = mx > m_run + kLazy ? mx : m_run;
+        const float alpha = m_new == m_run ? 1.f : exp2_fast(m_run - m_new);
+        m_run = m_new;
+        if (__any(alpha != 1.f)) {
+#pragma unroll
+            for (int dt = 0; dt < W::DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+        }
+        return alpha;
+    };
+    auto exp_pack = [&](f32x16& s, bf16x8 (&pf)[2]) {
+        const float mu = finite_max(m_run);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { s[i] = exp2_fast(MOD ? s[i] - mu : fmaf(s[i], p.scale_log2, -mu)); sum += s[i]; }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            u32x4 w;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) w[x] = pack16<F16>(s[8 * ks + 2 * x], s[8 * ks + 2 * x + 1]);
+            pf[ks] = __builtin_bit_cast(bf16x8, w);
+        }
+        return sum;
+    };
+    auto tile_max = [&](const f32x16& s) {
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        return mx;
+    };
+    // infinities and NaN of a tile's V fragments: out of the product, into the rows that see them
+    auto clean = [&](bf16x8 (&f)[W::KS], const int buf, const uint32_t bits) {
+        bool any = false;
+#pragma unroll
+        for (int s = 0; s < W::KS; ++s) any = any || frag_nonfinite<F16>(f[s]);
+        if (!__any(any)) return;
+#pragma unroll
+        for (int s = 0; s < W::KS; ++s) f[s] = frag_finite<F16>(f[s]);
+        for (int tk = 0; tk < 32; ++tk) {
+            if (!((bits >> tk) & 1u)) continue;
+            const uint8_t* vr = smem + (NBUF + buf) * W::TILEB + tk * W::ROWB + 8 * hh;
+#pragma unroll
+            for (int dt = 0; dt < W::DT; ++dt)
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const f32x4 e = nonfinite4<F16>(*reinterpret_cast<const uint2*>(vr + 16 * ((4 * dt + q4) ^ W::sV(tk))));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[dt][4 * q4 + i] += e[i];
+                }
+        }
+    };
+
+    auto pair_step = [&](const int k, auto pb_const) {
+        constexpr int pb = decltype(pb_const)::value, nb = 2 * (1 - pb);
+        wait_vmcnt<0>();                                           // pair k has landed
+        __syncthreads();                                           // ... everybody's part of it, and everyone left pair k - 1
+        int32_t sl[IPW];
+        const int base_a = 64 * k, base_b = 64 * k + 32;
+        if (base_a >= w_hi_max || base_a + 64 <= w_lo_min) {       // wave-uniform: nothing here for this wave's rows
+            pair_slots(k + 1, sl);
+#pragma unroll
+            for (int x = 0; x < IPW; ++x) { piece(false, x, sl[x], nb); piece(true, x, sl[x], nb); }
+            return;
+        }
+        bf16x8 fa[W::KS], fb[W::KS], pa[2], pbk[2];
+        f32x16 sa, sb;
+#pragma unroll
+        for (int s = 0; s < W::KS; ++s) fa[s] = rdk(2 * pb, s);
+        pair_slots(k + 1, sl);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { sa[i] = 0.f; sb[i] = 0.f; }
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int s = 0; s < W::KS; ++s) {                          // S_a^T; tile b's K fragments fill in behind
+            sa = mfma_32x32x16<F16>(fa[s], qf[s], sa);
+            fb[s] = rdk(2 * pb + 1, s);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < W::KS; ++s) {                          // S_b^T; tile a's V^T fragments take tile a's K registers
+            sb = mfma_32x32x16<F16>(fb[s], qf[s], sb);
+            fa[s] = rdv(2 * pb, s);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < IPW; ++x) piece(false, x, sl[x], nb);
+        if constexpr (MOD) { modify(sa, base_a); modify(sb, base_b); }
+        const bool part = base_a < w_lo_max || base_a + 64 > w_hi_min;      // wave-uniform
+        uint32_t bits_a = 0, bits_b = 0;
+        if (part) {
+            bits_a = row_bits(p, r, t, lo, hi, base_a);
+            bits_b = row_bits(p, r, t, lo, hi, base_b);
+            mask(sa, bits_a);
+            mask(sb, bits_b);
+        }
+        const float alpha = new_max(fmaxf(tile_max(sa), tile_max(sb)));
+        if (part) clean(fa, 2 * pb, bits_a);
+#pragma unroll
+        for (int x = 0; x < IPW; ++x) piece(true, x, sl[x], nb);
+        float sum = exp_pack(sa, pa);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int s = 0; s < W::KS; ++s) {                          // O^T += V_a^T P_a^T; tile b's V^T fragments fill in behind
+            o[s >> 1] = mfma_32x32x16<F16>(fa[s], pa[s & 1], o[s >> 1]);
+            fb[s] = rdv(2 * pb + 1, s);
+        }
+        sum += exp_pack(sb, pbk);                                  // independent of the MFMAs above: interleaved with them
+        __builtin_amdgcn_sched_barrier(0);
+        if (part) clean(fb, 2 * pb + 1, bits_b);
+#pragma unroll
+        for (int s = 0; s < W::KS; ++s) o[s >> 1] = mfma_32x32x16<F16>(fb[s], pbk[s & 1], o[s >> 1]);
+        __builtin_amdgcn_s_setprio(0);
+        l_run = fmaf(l_run, alpha, sum);
+    };
+    if (!none) {
+        fill_slots((2 * p_begin) / (kSlotWin / 32));
+        int32_t sl[IPW];
+        pair_slots(p_begin, sl);
+#pragma unroll
+        for (int x = 0; x < IPW; ++x) { piece(false, x, sl[x], 0); piece(true, x, sl[x], 0); }
+        for (int k0 = p_begin; k0 < n_pairs; k0 += 2) {
+            pair_step(k0, IntC<0>{});
+            if (k0 + 1 < n_pairs) pair_step(k0 + 1, IntC<1>{});
+        }
+        wait_vmcnt<0>();                                           // the repeated fetch of the last pair must not outlive the wave
+    }
+
+    float la, lb;
+    lane_pair<32>(l_run, la, lb);
+    const float lt = la + lb;
+    const int64_t item = t * p.Hq + h * p.G + g;
+    if (!valid) return;
+    if (p.splits > 1 && sp == 0 && hh == 0) p.part_n[item] = active;
+    if (active > 1) {                                              // unnormalised partial of this split: O^T, m, l
+        float* wo = p.part + (item * p.splits + sp) * (D + 4);
+#pragma unroll
+        for (int dt = 0; dt < W::DT; ++dt)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+                *reinterpret_cast<f32x4*>(wo + 32 * dt + 8 * q4 + 4 * hh) =
+                    f32x4{o[dt][4 * q4 + 0], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
+        if (hh == 0) { wo[D] = m_run; wo[D + 1] = lt; }
+        return;
+    }
+    const float inv = 1.f / lt;
+    uint16_t* op = p.out + t * p.o_stride + (int64_t)(h * p.G + g) * D + 4 * hh;
+#pragma unroll
+    for (int dt = 0; dt < W::DT; ++dt)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            uint2 w = {0u, 0u};
+            if (lt != 0.f) w = make_uint2(pack16<F16>(o[dt][4 * q4 + 0] * inv, o[dt][4 * q4 + 1] * inv),
+                                          pack16<F16>(o[dt][4 * q4 + 2] * inv, o[dt][4 * q4 + 3] * inv));
+            *reinterpret_cast<uint2*>(op + 32 * dt + 8 * q4) = w;
+        }
+}
+
+// out[row, head, :] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the splits that hold a part: D/4 lanes per (row, head),
+// four floats each, eight splits' loads in flight per lane.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void scored_merge_kernel(const ScoredParams p) {
+    constexpr int LPI = D / 4, CH = 8;
+    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPI;
+    const int li = threadIdx.x % LPI;
+    const int64_t row = item / p.Hq, head = item - row * p.Hq;
+    const int64_t r0 = p.cu_q ? imax(p.cu_q[0], 0) : 0, r1 = p.cu_q ? imin(p.cu_q[p.B], p.T) : imin(p.B, p.T);
+    if (row < r0 || row >= r1) return;                              // rows of no request: left as they were
+    const int n = imin(p.part_n[item], p.splits);
+    if (n <= 1) return;                                             // written by the attention kernel
+    const float* base = p.part + item * p.splits * (D + 4);
+    float mx = -INFINITY, den = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < n; s0 += CH) {
+        float m[CH], l[CH];
+        f32x4 o[CH];
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+            const float* ps = base + (int64_t)imin(s0 + k, n - 1) * (D + 4);
+            const float2 ml = *reinterpret_cast<const float2*>(ps + D);
+            m[k] = s0 + k < n ? ml.x : -INFINITY;
+            l[k] = s0 + k < n ? ml.y : 0.f;
+            o[k] = *reinterpret_cast<const f32x4*>(ps + 4 * li);
+            if (s0 + k >= n) o[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        float mn = mx;
+#pragma unroll
+        for (int k = 0; k < CH; ++k) mn = fmaxf(mn, m[k]);
+        const float mu = finite_max(mn), rs = exp2_fast(mx - mu);
+        den *= rs;
+        acc *= rs;
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+            const float w = exp2_fast(m[k] - mu);
+            den = fmaf(w, l[k], den);
+            acc += o[k] * w;
+        }
+        mx = mn;
+    }
+    const float inv = 1.f / den;
+    uint2 w = {0u, 0u};
+    if (den != 0.f) w = make_uint2(pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv));
+    *reinterpret_cast<uint2*>(p.out + row * p.o_stride + head * D + 4 * li) = w;
+}
+
+// ------------------------------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------------------------------
 static int shift_of(int32_t x) {
     if (x <= 0 || (x & (x - 1))) return -1;
     int s = 0;
@@ -93,13 +748,47 @@ static int shift_of(int32_t x) {
     return s;
 }
 
+// How a call is cut, from its sizes alone (so that the workspace query and the launch agree).
+struct ScoredCut { bool wide; int rt; int32_t blocks, splits, chunk; int64_t part_bytes, bytes; };
+static ScoredCut scored_cut(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int32_t D, int64_t ext, int64_t max_len, int64_t window) {
+    ScoredCut c = {};
+    const int64_t G = Hq / Hkv;
+    if (ext > T) ext = T;
+    const int64_t rows = ext * G;
+    c.wide = rows > 64;
+    c.rt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+    const int64_t per_block = c.wide ? 128 : 16 * c.rt;
+    c.blocks = (int32_t)((rows + per_block - 1) / per_block);
+    int64_t span = window > 0 && window + ext < max_len ? window + ext : max_len;
+    span += c.wide ? 63 : 31;                                       // the first tile may begin before the first visible key
+    // workgroups there are without splits (a ragged batch has fewer row blocks than its longest request suggests)
+    int64_t units = B * Hkv * c.blocks;
+    const int64_t packed = Hkv * ((T * G + per_block - 1) / per_block + B);
+    if (packed < units) units = packed;
+    const int64_t target = c.wide || D == 128 ? 512 : 1024, shortest = c.wide ? 512 : 128;
+    int64_t splits = target / units;
+    if (splits < 1) splits = 1;
+    int64_t chunk = (span + splits - 1) / splits;
+    if (chunk < shortest) chunk = shortest;
+    if (!c.wide && chunk > kFewSlots) chunk = kFewSlots;
+    chunk = (chunk + 63) / 64 * 64;
+    splits = (span + chunk - 1) / chunk;
+    c.splits = (int32_t)splits;
+    c.chunk = (int32_t)chunk;
+    if (splits > 1) {
+        c.part_bytes = T * Hq * splits * (D + 4) * (int64_t)sizeof(float);
+        c.bytes = c.part_bytes + T * Hq * (int64_t)sizeof(int32_t);
+    }
+    return c;
+}
+
 // what both entry points refuse
-static int check_common(const ScoredParams& p, int32_t max_extend_len, int32_t max_seq_len, int32_t D, int32_t dtype) {
+static int check_common(const ScoredParams& p, int32_t max_extend_len, int32_t max_seq_len, int32_t D, float scale, float cap, int32_t dtype) {
     if (!p.q || !p.k_pool || !p.v_pool || !p.page_table || !p.page_table_ids || !p.out) return M355_ERR_INVALID_ARG;
     if (p.B < 0 || p.T < 0 || p.Hq <= 0 || p.Hkv <= 0 || p.Hq % p.Hkv || p.ps <= 0 || p.pt_rows <= 0 || p.pt_cols <= 0) return M355_ERR_INVALID_ARG;
     if (p.S <= 0 || p.S > 0x7fffffffLL || p.pt_stride < p.pt_cols || (int64_t)p.pt_cols * p.ps > 0x3fffffffLL) return M355_ERR_INVALID_ARG;
     if (max_extend_len <= 0 || max_seq_len <= 0 || p.window < 0) return M355_ERR_INVALID_ARG;
-    if (!(p.scale > 0.f) || !(p.scale < 1e30f) || !(p.cap >= 0.f) || !(p.cap < 1e30f)) return M355_ERR_INVALID_ARG;
+    if (!(scale > 0.f) || !(scale < 1e30f) || !(cap >= 0.f) || !(cap < 1e30f)) return M355_ERR_INVALID_ARG;
     if (dtype != M355_DTYPE_BF16 && dtype != M355_DTYPE_F16) return M355_ERR_UNSUPPORTED;
     if (D != 64 && D != 128) return M355_ERR_UNSUPPORTED;
     if (p.row_elems < (int64_t)p.Hkv * D || p.row_elems % 8) return M355_ERR_INVALID_ARG;
@@ -108,15 +797,41 @@ static int check_common(const ScoredParams& p, int32_t max_extend_len, int32_t m
     return M355_OK;
 }
 
-static int launch_scored(const ScoredParams& p, int32_t max_extend_len, int32_t D, int32_t dtype, void* stream) {
-    const dim3 grid((unsigned)max_extend_len, (unsigned)p.Hq, (unsigned)p.B);
+template <int D, bool MOD, bool F16>
+static void launch_kernels(const ScoredParams& p, const ScoredCut& c, hipStream_t st) {
+    if (c.wide) {
+        hipLaunchKernelGGL((scored_wide_kernel<D, MOD, F16>), dim3((unsigned)(p.B * p.Hkv * p.blocks), (unsigned)p.splits), dim3(256), 0, st, p);
+    } else {
+        const int64_t units = (int64_t)p.splits * p.B * p.Hkv;
+        const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.blocks));
+        if (c.rt == 1) hipLaunchKernelGGL((scored_few_kernel<D, 1, MOD, F16>), grid, dim3(256), 0, st, p);
+        else if (c.rt == 2) hipLaunchKernelGGL((scored_few_kernel<D, 2, MOD, F16>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((scored_few_kernel<D, 4, MOD, F16>), grid, dim3(256), 0, st, p);
+    }
+    if (p.splits > 1) {
+        const int64_t lanes = (int64_t)p.T * p.Hq * (D / 4);
+        hipLaunchKernelGGL((scored_merge_kernel<D, F16>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, p);
+    }
+}
+
+static int launch_scored(ScoredParams& p, int32_t max_extend_len, int32_t max_seq_len, int32_t D, float scale, float cap, int32_t dtype,
+                         void* workspace, int64_t workspace_bytes, void* stream) {
+    if (const int e = check_common(p, max_extend_len, max_seq_len, D, scale, cap, dtype)) return e;
+    const ScoredCut c = scored_cut(p.B, p.T, p.Hq, p.Hkv, D, max_extend_len, max_seq_len, p.window);
+    if (c.bytes && (!workspace || workspace_bytes < c.bytes || ((uintptr_t)workspace & 255))) return M355_ERR_WORKSPACE;
+    if ((int64_t)p.B * p.Hkv * c.blocks * (c.wide ? 1 : c.splits) > 0x3fffffffLL || c.splits > 65535 ||
+        (int64_t)p.T * p.Hq * (D / 4) / 256 > 0x3fffffffLL) return M355_ERR_INVALID_ARG;
+    p.G = p.Hq / p.Hkv; p.ps_shift = shift_of(p.ps);
+    p.scale_log2 = scale * kLog2e; p.cap_log2 = cap * kLog2e; p.cap_rate = cap > 0.f ? 2.f * scale * kLog2e / cap : 0.f;
+    p.blocks = c.blocks; p.splits = c.splits; p.chunk = c.chunk;
+    if (c.bytes) { p.part = (float*)workspace; p.part_n = (int32_t*)((uint8_t*)workspace + c.part_bytes); }
     hipStream_t st = (hipStream_t)stream;
-    const bool f16 = dtype == M355_DTYPE_F16;
-    if (D == 64 && f16) hipLaunchKernelGGL((scored_rows_kernel<64, true>), grid, dim3(64), 0, st, p);
-    else if (D == 64) hipLaunchKernelGGL((scored_rows_kernel<64, false>), grid, dim3(64), 0, st, p);
-    else if (f16) hipLaunchKernelGGL((scored_rows_kernel<128, true>), grid, dim3(64), 0, st, p);
-    else hipLaunchKernelGGL((scored_rows_kernel<128, false>), grid, dim3(64), 0, st, p);
-    return check_launch();
+    const bool mod = cap > 0.f || p.slopes, f16 = dtype == M355_DTYPE_F16;
+#define M355_SCORED(DD, MM, FF) if (D == DD && mod == MM && f16 == FF) { launch_kernels<DD, MM, FF>(p, c, st); return check_launch(); }
+    M355_SCORED(64, false, false) M355_SCORED(64, false, true) M355_SCORED(64, true, false) M355_SCORED(64, true, true)
+    M355_SCORED(128, false, false) M355_SCORED(128, false, true) M355_SCORED(128, true, false) M355_SCORED(128, true, true)
+#undef M355_SCORED
+    return M355_ERR_UNSUPPORTED;
 }
 
 }  // namespace m355
@@ -125,7 +840,8 @@ using namespace m355;
 
 extern "C" int64_t m355_scored_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_extend_len,
                                                int32_t max_seq_len_hint, int32_t window) {
-    return 0;
+    if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_extend_len <= 0 || max_seq_len_hint <= 0 || window < 0) return 0;
+    return scored_cut(B, T, Hq, Hkv, D, max_extend_len, max_seq_len_hint, window).bytes;
 }
 
 extern "C" int m355_scored_attn(const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool, int64_t pool_row_stride,
@@ -136,19 +852,15 @@ extern "C" int m355_scored_attn(const void* q, int64_t q_row_stride, const void*
                                 float softcap, const float* slopes, int32_t window, const int32_t* doc_starts,
                                 const int32_t* bidir_lens, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream) {
     if (T == 0 || B == 0) return M355_OK;
-    if (!seq_lens || (prefix_lens == nullptr) != (cu_q == nullptr)) return M355_ERR_INVALID_ARG;
+    if (!seq_lens || (prefix_lens == nullptr) != (cu_q == nullptr) || (!cu_q && T < B)) return M355_ERR_INVALID_ARG;
     ScoredParams p = {};
     p.q = (const uint16_t*)q; p.k_pool = (const uint16_t*)k_pool; p.v_pool = (const uint16_t*)v_pool;
     p.page_table = page_table; p.page_table_ids = page_table_ids; p.seq_lens = seq_lens; p.prefix_lens = prefix_lens; p.cu_q = cu_q;
     p.out = (uint16_t*)out; p.q_stride = q_row_stride; p.o_stride = o_row_stride;
     p.row_elems = pool_row_stride ? pool_row_stride : (int64_t)Hkv * D;
     p.pt_stride = pt_row_stride; p.S = S; p.pt_rows = pt_rows; p.pt_cols = pt_cols; p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv;
-    p.ps = page_size; p.scale = scale; p.cap = softcap; p.slopes = slopes; p.window = window;
-    p.doc_starts = doc_starts; p.bidir = bidir_lens;
-    if (!cu_q && T < B) return M355_ERR_INVALID_ARG;
-    if (const int e = check_common(p, max_extend_len, max_seq_len_hint, D, dtype)) return e;
-    p.G = Hq / Hkv; p.ps_shift = shift_of(page_size);
-    return launch_scored(p, cu_q ? max_extend_len : 1, D, dtype, stream);
+    p.ps = page_size; p.slopes = slopes; p.window = window; p.doc_starts = doc_starts; p.bidir = bidir_lens;
+    return launch_scored(p, cu_q ? max_extend_len : 1, max_seq_len_hint, D, scale, softcap, dtype, workspace, workspace_bytes, stream);
 }
 
 extern "C" int m355_tree_attn(const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool, int64_t pool_row_stride,
@@ -167,9 +879,6 @@ extern "C" int m355_tree_attn(const void* q, int64_t q_row_stride, const void* k
     p.out = (uint16_t*)out; p.q_stride = q_row_stride; p.o_stride = o_row_stride;
     p.row_elems = pool_row_stride ? pool_row_stride : (int64_t)Hkv * D;
     p.pt_stride = pt_row_stride; p.S = S; p.pt_rows = pt_rows; p.pt_cols = pt_cols; p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv;
-    p.ps = page_size; p.scale = scale; p.cap = softcap; p.slopes = slopes;
-    p.mask = tree_mask; p.words = mask_words; p.positions = positions;
-    if (const int e = check_common(p, max_nodes, max_seq_len_hint, D, dtype)) return e;
-    p.G = Hq / Hkv; p.ps_shift = shift_of(page_size);
-    return launch_scored(p, max_nodes, D, dtype, stream);
+    p.ps = page_size; p.slopes = slopes; p.mask = tree_mask; p.words = mask_words; p.positions = positions;
+    return launch_scored(p, max_nodes, max_seq_len_hint, D, scale, softcap, dtype, workspace, workspace_bytes, stream);
 }
