@@ -133,12 +133,18 @@ def check(code: int, what: str) -> None:
         raise MI355AttnError(f"{what} failed: {msg} (code {code})")
 
 
+_dtype_codes = {}                    # filled on first use: torch is imported by the callers, not here
+
+
 def dtype_code(torch_dtype) -> int:
-    import torch
-    try:
-        return {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}[torch_dtype]
-    except KeyError:
-        raise MI355AttnError(f"unsupported dtype {torch_dtype}") from None
+    code = _dtype_codes.get(torch_dtype)
+    if code is None:
+        import torch
+        _dtype_codes.update({torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32})
+        code = _dtype_codes.get(torch_dtype)
+        if code is None:
+            raise MI355AttnError(f"unsupported dtype {torch_dtype}")
+    return code
 
 
 def require_cuda(t, name: str):

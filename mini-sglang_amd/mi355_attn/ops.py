@@ -4,6 +4,7 @@ Every argument tensor must be on the GPU; results are enqueued on torch's curren
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional
 
@@ -388,53 +389,91 @@ def rope_kv_store(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, hea
 
 
 # ---- attention with modified scores, trees of drafted tokens, log probabilities -----------------------------------------
-def _device_of(tensors) -> None:
+# (These calls sit on the path of every layer of every step, so their checks are written for few interpreter steps: a wrapper that
+# took 20 us of host time would be longer than most of the launches behind it.)
+def _on_device(*named) -> None:
     """Every tensor on the GPU that is current: the launch goes to its stream, and kernels of one device must not be handed
-    another's memory."""
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    for n, t in tensors:
-        require_cuda(t, n)
-        if t.device.index != dev:
-            raise _lib.MI355AttnError(f"{n} is on {t.device}, the current device is cuda:{dev} (use torch.cuda.device)")
+    another's memory.  `named`: name, tensor, name, tensor, ...; None is skipped."""
+    dev = None
+    for name, t in zip(named[::2], named[1::2]):
+        if t is None:
+            continue
+        at = t.get_device()
+        if at < 0:
+            require_cuda(t, name)
+        if dev is None:
+            dev = torch.cuda.current_device()
+        if at != dev:
+            raise _lib.MI355AttnError(f"{name} is on {t.device}, the current device is cuda:{dev} (use torch.cuda.device)")
 
 
-def _vector(name: str, t, dtype, n: int) -> None:
-    if t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+def _vector(name: str, t, dtype, n: int) -> int:
+    """The address of a contiguous vector of n elements."""
+    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
         raise _lib.MI355AttnError(f"{name} must be a contiguous {dtype} vector of {n}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
 
 
-def _scored_buffers(what: str, q, k_pool, v_pool, page_table, num_heads: int, page_size: int, out, workspace, need: int):
-    """Shapes, types and strides that both scored entry points share.  Returns (q rows, pool pitch, out, workspace)."""
-    if k_pool.dim() != 3 or q.dim() < 2:
-        raise _lib.MI355AttnError(f"{what}: q must be [T, heads*D], the pools [S, Hkv, D]")
-    S, Hkv, D = k_pool.shape
+def _rows(what: str, q: torch.Tensor, width: int) -> torch.Tensor:
+    """q as [T, width] rows that the kernels can read: inner stride 1, rows 16-byte aligned."""
     T = q.shape[0]
-    if q.dtype != k_pool.dtype or q.dtype != v_pool.dtype:
+    if q.numel() != T * width:
+        raise _lib.MI355AttnError(f"{what}: q {tuple(q.shape)} is not [T, {width}]")
+    if q.dim() != 2:
+        q = q.reshape(T, width)
+    if T and (q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16):
+        q = q.contiguous() if not q.is_contiguous() else q.clone()
+    return q
+
+
+def _pools(what: str, q, k_pool, v_pool):
+    """(S, Hkv, D, row pitch) of the pools, which share layout and dtype with each other and dtype with q."""
+    shape, stride = k_pool.shape, k_pool.stride()
+    if len(shape) != 3 or v_pool.shape != shape or v_pool.stride() != stride or stride[2] != 1 or (stride[1] != shape[2] and shape[1] > 1):
+        raise _lib.MI355AttnError(f"{what}: KV pools must be [S, Hkv, D], dense inside a row, K and V with the same row pitch")
+    if q.dtype is not k_pool.dtype or q.dtype is not v_pool.dtype:
         raise _lib.MI355AttnError(f"{what}: q and the pools must have one dtype, got {q.dtype}, {k_pool.dtype}, {v_pool.dtype}")
-    if num_heads <= 0 or num_heads % Hkv or q.numel() != T * num_heads * D:
-        raise _lib.MI355AttnError(f"{what}: q {tuple(q.shape)} is not [T, {num_heads} * {D}], a multiple of {Hkv} kv heads")
-    q2 = q.reshape(T, num_heads * D)
-    if T and (q2.stride(1) != 1 or q2.stride(0) % 8 or q2.data_ptr() % 16):
-        q2 = q2.contiguous()
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 or page_size < 1:
-        raise _lib.MI355AttnError(f"{what}: page_table must be int32 [rows, pages] with inner stride 1, page_size >= 1")
+    S, Hkv, D = shape
+    pitch = stride[0] if S > 1 else Hkv * D
+    if pitch < Hkv * D or pitch % 8:
+        raise _lib.MI355AttnError(f"{what}: KV pool row pitch {pitch} must be a multiple of 8 elements and >= Hkv*D")
+    return S, Hkv, D, pitch
+
+
+def _table(what: str, page_table, page_size: int):
+    """(rows, columns, row stride) of a page table."""
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_size < 1:
+        raise _lib.MI355AttnError(f"{what}: page_table must be int32 [rows, pages], page_size >= 1")
+    rows, cols = page_table.shape
+    s0, s1 = page_table.stride()
+    if s1 != 1 and cols > 1:
+        raise _lib.MI355AttnError(f"{what}: page_table must have inner stride 1")
+    return rows, cols, s0 if rows > 1 else max(cols, s0)
+
+
+def _out_rows(what: str, q, out, T: int, width: int):
     if out is None:
-        out = torch.empty((T, num_heads * D), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or tuple(out.shape) != (T, num_heads * D) or (T and out.stride(1) != 1):
+        return q.new_empty((T, width)), width
+    if out.dtype is not q.dtype or out.shape != (T, width) or (T and out.stride(1) != 1):
         raise _lib.MI355AttnError(f"{what}: out must be {q.dtype} [T, heads*D] with inner stride 1")
-    elif T and out.data_ptr() == q2.data_ptr():
+    if T and out.data_ptr() == q.data_ptr():
         raise _lib.MI355AttnError(f"{what}: out must not be q")
+    return out, out.stride(0) if T > 1 else max(width, out.stride(0))
+
+
+def _scratch(workspace, need: int, device):
+    """(tensor that owns it, address, bytes) of a call's workspace: the caller's, or a new one of `need` bytes."""
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    elif not workspace.is_contiguous():
-        raise _lib.MI355AttnError(f"{what}: workspace must be contiguous")
-    return q2, pool_pitch(k_pool, v_pool), out, workspace
+        if not need:
+            return None, None, 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        return workspace, workspace.data_ptr(), need
+    if not workspace.is_contiguous():
+        raise _lib.MI355AttnError("workspace must be contiguous")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
-def _stride0(t, width: int) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(width, t.stride(0))
-
-
+@functools.lru_cache(maxsize=4096)
 def scored_workspace_bytes(B: int, T: int, Hq: int, Hkv: int, D: int, max_extend_len: int, max_seq_len: int, window: int = 0) -> int:
     return int(_lib.load().m355_scored_workspace_bytes(B, T, Hq, Hkv, D, max_extend_len, max_seq_len, window))
 
@@ -454,39 +493,37 @@ def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, pag
     With prefix_lens (int64 [B]) and cu_q (int32 [B+1]): ragged rows over cached prefixes, as prefill_attn; rows of q at or past
     cu_q[B] are left as they were in `out`.  Without them: one row per request, its newest token at seq_lens - 1.  A row that
     sees nothing gives zeros."""
-    lib = _lib.load()
-    given = [("q", q), ("k_pool", k_pool), ("v_pool", v_pool), ("page_table", page_table), ("page_table_ids", page_table_ids),
-             ("seq_lens", seq_lens)]
-    given += [(n, t) for n, t in (("prefix_lens", prefix_lens), ("cu_q", cu_q), ("slopes", slopes), ("doc_starts", doc_starts),
-                                  ("bidir_lens", bidir_lens), ("workspace", workspace), ("out", out)) if t is not None]
-    _device_of(given)
-    B, T = seq_lens.numel(), q.shape[0]
-    if (prefix_lens is None) != (cu_q is None):
+    _on_device("q", q, "k_pool", k_pool, "v_pool", v_pool, "page_table", page_table, "page_table_ids", page_table_ids, "seq_lens", seq_lens,
+               "prefix_lens", prefix_lens, "cu_q", cu_q, "slopes", slopes, "doc_starts", doc_starts, "bidir_lens", bidir_lens,
+               "workspace", workspace, "out", out)
+    B, T, max_seq_len, max_extend_len = seq_lens.numel(), q.shape[0], int(max_seq_len), int(max_extend_len)
+    S, Hkv, D, pitch = _pools("scored_attn", q, k_pool, v_pool)
+    pt_rows, pt_cols, pt_stride = _table("scored_attn", page_table, page_size)
+    lens, ids = _vector("seq_lens", seq_lens, torch.int64, B), _vector("page_table_ids", page_table_ids, torch.int64, B)
+    pre = cu = None
+    if cu_q is not None and prefix_lens is not None:
+        pre, cu = _vector("prefix_lens", prefix_lens, torch.int64, B), _vector("cu_q", cu_q, torch.int32, B + 1)
+    elif cu_q is not None or prefix_lens is not None:
         raise _lib.MI355AttnError("scored_attn: prefix_lens and cu_q go together (neither: one row per request)")
-    _vector("seq_lens", seq_lens, torch.int64, B), _vector("page_table_ids", page_table_ids, torch.int64, B)
-    if cu_q is not None:
-        _vector("prefix_lens", prefix_lens, torch.int64, B), _vector("cu_q", cu_q, torch.int32, B + 1)
-    elif T != B:
-        raise _lib.MI355AttnError(f"scored_attn: {T} rows for {B} requests (pass prefix_lens and cu_q for more than one row each)")
-    if slopes is not None:
-        _vector("slopes", slopes, torch.float32, num_heads)
-    if doc_starts is not None:
-        _vector("doc_starts", doc_starts, torch.int32, T)
-    if bidir_lens is not None:
-        _vector("bidir_lens", bidir_lens, torch.int32, B)
-    if cu_q is None:
+    else:
         max_extend_len = 1
-    D = k_pool.shape[-1]
-    need = scored_workspace_bytes(B, T, num_heads, k_pool.shape[1], D, max_extend_len, max_seq_len, window) if workspace is None else 0
-    q2, pitch, out, workspace = _scored_buffers("scored_attn", q, k_pool, v_pool, page_table, num_heads, page_size, out, workspace, need)
+        if T != B:
+            raise _lib.MI355AttnError(f"scored_attn: {T} rows for {B} requests (pass prefix_lens and cu_q for more than one row each)")
+    slope_ptr = None if slopes is None else _vector("slopes", slopes, torch.float32, num_heads)
+    doc_ptr = None if doc_starts is None else _vector("doc_starts", doc_starts, torch.int32, T)
+    bidir_ptr = None if bidir_lens is None else _vector("bidir_lens", bidir_lens, torch.int32, B)
     W = num_heads * D
-    check(lib.m355_scored_attn(q2.data_ptr(), _stride0(q2, W), k_pool.data_ptr(), v_pool.data_ptr(), pitch, k_pool.shape[0],
-                               page_table.data_ptr(), _stride0(page_table, page_table.shape[1]), page_table.shape[0], page_table.shape[1],
-                               page_table_ids.data_ptr(), seq_lens.data_ptr(), _ptr(prefix_lens), _ptr(cu_q), out.data_ptr(),
-                               _stride0(out, W), B, T, max_extend_len, max_seq_len, num_heads, k_pool.shape[1], D, page_size,
-                               float(D) ** -0.5 if scale is None else scale, softcap, _ptr(slopes), window, _ptr(doc_starts),
-                               _ptr(bidir_lens), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
-                               dtype_code(q.dtype), current_stream()), "m355_scored_attn")
+    q2 = _rows("scored_attn", q, W)
+    out, o_stride = _out_rows("scored_attn", q2, out, T, W)
+    need = 0 if workspace is not None else scored_workspace_bytes(B, T, num_heads, Hkv, D, max_extend_len, max_seq_len, window)
+    held, ws_ptr, ws_bytes = _scratch(workspace, need, q.device)
+    code = _lib.load().m355_scored_attn(q2.data_ptr(), q2.stride(0) if T > 1 else W, k_pool.data_ptr(), v_pool.data_ptr(), pitch, S,
+                                        page_table.data_ptr(), pt_stride, pt_rows, pt_cols, ids, lens, pre, cu, out.data_ptr(), o_stride,
+                                        B, T, max_extend_len, max_seq_len, num_heads, Hkv, D, page_size,
+                                        D ** -0.5 if scale is None else scale, softcap, slope_ptr, window, doc_ptr, bidir_ptr, ws_ptr,
+                                        ws_bytes, dtype_code(q.dtype), current_stream())
+    if code:
+        check(code, "m355_scored_attn")
     return out
 
 
@@ -505,34 +542,30 @@ def tree_prepare(page_table: torch.Tensor, page_table_ids: torch.Tensor, prefix_
     """Metadata of a batch of draft trees, one launch (m355_tree_prepare): ancestor masks, positions and slots of all nodes, and
     the page-table entries of new_pages (int32; request b owns new_pages[new_page_off[b]:new_page_off[b+1]], behind the pages of
     its prefix).  parents int32 [T]: index of the parent inside the request, below the node's own, or -1."""
-    lib = _lib.load()
-    given = [("page_table", page_table), ("page_table_ids", page_table_ids), ("prefix_lens", prefix_lens), ("parents", parents),
-             ("cu_q", cu_q)]
+    _on_device("page_table", page_table, "page_table_ids", page_table_ids, "prefix_lens", prefix_lens, "parents", parents, "cu_q", cu_q,
+               "new_pages", new_pages, "new_page_off", new_page_off)
+    B, T = prefix_lens.numel(), parents.numel()
+    pt_rows, pt_cols, pt_stride = _table("tree_prepare", page_table, page_size)
+    ids, pre = _vector("page_table_ids", page_table_ids, torch.int64, B), _vector("prefix_lens", prefix_lens, torch.int64, B)
+    par, cu = _vector("parents", parents, torch.int32, T), _vector("cu_q", cu_q, torch.int32, B + 1)
+    fresh = off = None
     if (new_pages is None) != (new_page_off is None):
         raise _lib.MI355AttnError("tree_prepare: new_pages and new_page_off go together")
     if new_pages is not None:
-        given += [("new_pages", new_pages), ("new_page_off", new_page_off)]
-    _device_of(given)
-    B, T = prefix_lens.numel(), parents.numel()
-    _vector("page_table_ids", page_table_ids, torch.int64, B), _vector("prefix_lens", prefix_lens, torch.int64, B)
-    _vector("parents", parents, torch.int32, T), _vector("cu_q", cu_q, torch.int32, B + 1)
-    if new_pages is not None:
-        _vector("new_pages", new_pages, torch.int32, new_pages.numel()), _vector("new_page_off", new_page_off, torch.int32, B + 1)
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 or page_size < 1:
-        raise _lib.MI355AttnError("tree_prepare: page_table must be int32 [rows, pages] with inner stride 1, page_size >= 1")
+        n = new_pages.numel()
+        fresh, off = _vector("new_pages", new_pages, torch.int32, n), _vector("new_page_off", new_page_off, torch.int32, B + 1)
+        if n == 0:                                          # (no address: the table is complete)
+            fresh = off = None
     if not 1 <= max_nodes <= _lib.TREE_MAX_NODES:
         raise _lib.MI355AttnError(f"tree_prepare: trees of 1 to {_lib.TREE_MAX_NODES} nodes are supported, got max_nodes {max_nodes}")
-    words = -(-max_nodes // 32)
-    dev = parents.device
-    mask = torch.empty((T, words), dtype=torch.int32, device=dev)
-    two = torch.empty((2, T), dtype=torch.int64, device=dev)
-    # (an empty new_pages has no address: the table is complete then)
-    fresh = new_pages is not None and new_pages.numel() > 0
-    check(lib.m355_tree_prepare(page_table.data_ptr(), _stride0(page_table, page_table.shape[1]), page_table.shape[0], page_table.shape[1],
-                                page_table_ids.data_ptr(), prefix_lens.data_ptr(), parents.data_ptr(), cu_q.data_ptr(),
-                                new_pages.data_ptr() if fresh else None, new_page_off.data_ptr() if fresh else None, B, T, max_nodes,
-                                page_size, mask.data_ptr(), words, two[0].data_ptr(), two[1].data_ptr(), current_stream()), "m355_tree_prepare")
-    return TreePlan(mask, two[0], two[1], cu_q, max_nodes)
+    words = (max_nodes + 31) // 32
+    mask = parents.new_empty((T, words))
+    positions, slots = prefix_lens.new_empty((2, T)).unbind()
+    code = _lib.load().m355_tree_prepare(page_table.data_ptr(), pt_stride, pt_rows, pt_cols, ids, pre, par, cu, fresh, off, B, T, max_nodes,
+                                         page_size, mask.data_ptr(), words, positions.data_ptr(), slots.data_ptr(), current_stream())
+    if code:
+        check(code, "m355_tree_prepare")
+    return TreePlan(mask, positions, slots, cu_q, max_nodes)
 
 
 def tree_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
@@ -542,30 +575,29 @@ def tree_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_
     """Attention of drafted nodes over the cached prefix and their ancestors (m355_tree_attn), after the nodes' K/V have been
     written to plan.out_cache_loc.  max_seq_len >= the longest prefix + nodes; softcap / slopes as scored_attn, distances between
     nodes being differences of depth."""
-    lib = _lib.load()
-    given = [("q", q), ("k_pool", k_pool), ("v_pool", v_pool), ("page_table", page_table), ("page_table_ids", page_table_ids),
-             ("prefix_lens", prefix_lens), ("mask", plan.mask), ("positions", plan.positions), ("cu_q", plan.cu_q)]
-    given += [(n, t) for n, t in (("slopes", slopes), ("workspace", workspace), ("out", out)) if t is not None]
-    _device_of(given)
-    B, T = prefix_lens.numel(), q.shape[0]
-    _vector("page_table_ids", page_table_ids, torch.int64, B), _vector("prefix_lens", prefix_lens, torch.int64, B)
-    _vector("plan.cu_q", plan.cu_q, torch.int32, B + 1), _vector("plan.positions", plan.positions, torch.int64, T)
-    if plan.mask.dtype != torch.int32 or plan.mask.dim() != 2 or plan.mask.shape[0] != T or not plan.mask.is_contiguous():
-        raise _lib.MI355AttnError(f"tree_attn: the plan is for {plan.mask.shape[0]} nodes, q has {T} rows")
-    if slopes is not None:
-        _vector("slopes", slopes, torch.float32, num_heads)
-    D = k_pool.shape[-1]
-    need = scored_workspace_bytes(B, T, num_heads, k_pool.shape[1], D, plan.max_nodes, max_seq_len) if workspace is None else 0
-    q2, pitch, out, workspace = _scored_buffers("tree_attn", q, k_pool, v_pool, page_table, num_heads, page_size, out, workspace, need)
+    mask, positions, cu_q = plan.mask, plan.positions, plan.cu_q
+    _on_device("q", q, "k_pool", k_pool, "v_pool", v_pool, "page_table", page_table, "page_table_ids", page_table_ids, "prefix_lens", prefix_lens,
+               "mask", mask, "positions", positions, "cu_q", cu_q, "slopes", slopes, "workspace", workspace, "out", out)
+    B, T, max_seq_len = prefix_lens.numel(), q.shape[0], int(max_seq_len)
+    S, Hkv, D, pitch = _pools("tree_attn", q, k_pool, v_pool)
+    pt_rows, pt_cols, pt_stride = _table("tree_attn", page_table, page_size)
+    ids, pre = _vector("page_table_ids", page_table_ids, torch.int64, B), _vector("prefix_lens", prefix_lens, torch.int64, B)
+    cu, pos_ptr = _vector("plan.cu_q", cu_q, torch.int32, B + 1), _vector("plan.positions", positions, torch.int64, T)
+    if mask.dtype is not torch.int32 or mask.dim() != 2 or mask.shape[0] != T or not mask.is_contiguous():
+        raise _lib.MI355AttnError(f"tree_attn: the plan is for {mask.shape[0]} nodes, q has {T} rows")
+    slope_ptr = None if slopes is None else _vector("slopes", slopes, torch.float32, num_heads)
     W = num_heads * D
-    check(lib.m355_tree_attn(q2.data_ptr(), _stride0(q2, W), k_pool.data_ptr(), v_pool.data_ptr(), pitch, k_pool.shape[0],
-                             page_table.data_ptr(), _stride0(page_table, page_table.shape[1]), page_table.shape[0], page_table.shape[1],
-                             page_table_ids.data_ptr(), prefix_lens.data_ptr(), plan.cu_q.data_ptr(), plan.mask.data_ptr(),
-                             plan.mask.shape[1], plan.positions.data_ptr(), out.data_ptr(), _stride0(out, W), B, T, plan.max_nodes,
-                             max_seq_len, num_heads, k_pool.shape[1], D, page_size, float(D) ** -0.5 if scale is None else scale,
-                             softcap, _ptr(slopes), _ptr(workspace),
-                             0 if workspace is None else workspace.numel() * workspace.element_size(), dtype_code(q.dtype),
-                             current_stream()), "m355_tree_attn")
+    q2 = _rows("tree_attn", q, W)
+    out, o_stride = _out_rows("tree_attn", q2, out, T, W)
+    need = 0 if workspace is not None else scored_workspace_bytes(B, T, num_heads, Hkv, D, plan.max_nodes, max_seq_len)
+    held, ws_ptr, ws_bytes = _scratch(workspace, need, q.device)
+    code = _lib.load().m355_tree_attn(q2.data_ptr(), q2.stride(0) if T > 1 else W, k_pool.data_ptr(), v_pool.data_ptr(), pitch, S,
+                                      page_table.data_ptr(), pt_stride, pt_rows, pt_cols, ids, pre, cu, mask.data_ptr(), mask.shape[1], pos_ptr,
+                                      out.data_ptr(), o_stride, B, T, plan.max_nodes, max_seq_len, num_heads, Hkv, D, page_size,
+                                      D ** -0.5 if scale is None else scale, softcap, slope_ptr, ws_ptr, ws_bytes, dtype_code(q.dtype),
+                                      current_stream())
+    if code:
+        check(code, "m355_tree_attn")
     return out
 
 
@@ -580,30 +612,36 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
                    workspace: Optional[torch.Tensor] = None) -> TokenLogprobs:
     """Log probabilities of `tokens` (int64 [T] or [T, n]; None: none) under softmax(logits / temperature), the rows' entropies
     and their top_k alternatives, ties to the lower id, in one pass over logits [T, V] (m355_token_logprobs)."""
-    lib = _lib.load()
-    _device_of([("logits", logits)] + [(n, t) for n, t in (("tokens", tokens), ("workspace", workspace)) if t is not None])
-    if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1):
+    _on_device("logits", logits, "tokens", tokens, "workspace", workspace)
+    if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1 and logits.shape[1] > 1):
         raise _lib.MI355AttnError(f"token_logprobs: logits must be [T, V] with inner stride 1, got {tuple(logits.shape)}")
     T, V = logits.shape
     if V < 1 or not 0 <= top_k <= min(V, _lib.MAX_TOP_LOGPROBS):
         raise _lib.MI355AttnError(f"token_logprobs: top_k {top_k} of a vocabulary of {V} (at most {_lib.MAX_TOP_LOGPROBS} are supported)")
     if not (temperature > 0 and math.isfinite(temperature)):
         raise _lib.MI355AttnError(f"token_logprobs: temperature must be positive, got {temperature}")
-    given, lp = 0, None
+    given, lp, tok_ptr, lp_ptr = 0, None, None, None
     if tokens is not None:
-        if tokens.dtype != torch.int64 or tokens.dim() not in (1, 2) or tokens.shape[0] != T:
+        if tokens.dtype is not torch.int64 or tokens.dim() not in (1, 2) or tokens.shape[0] != T:
             raise _lib.MI355AttnError(f"token_logprobs: tokens must be int64 [{T}] or [{T}, n], got {tokens.dtype} {tuple(tokens.shape)}")
         tokens = tokens.contiguous()
         given = 1 if tokens.dim() == 1 else tokens.shape[1]
-        lp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
-    entropy = torch.empty(T, dtype=torch.float32, device=logits.device)
-    top = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
-    ids = torch.empty((T, top_k), dtype=torch.int64, device=logits.device)
-    if workspace is None:
-        need = int(lib.m355_token_logprobs_workspace_bytes(T, V, top_k))
-        workspace = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
-    check(lib.m355_token_logprobs(logits.data_ptr(), logits.stride(0) if T > 1 else max(V, logits.stride(0)), _ptr(tokens), given, T, V, top_k,
-                                  temperature, _ptr(lp), entropy.data_ptr(), top.data_ptr(), ids.data_ptr(), _ptr(workspace),
-                                  0 if workspace is None else workspace.numel() * workspace.element_size(), dtype_code(logits.dtype),
-                                  current_stream()), "m355_token_logprobs")
+        lp = torch.empty_like(tokens, dtype=torch.float32)
+        if given:
+            tok_ptr, lp_ptr = tokens.data_ptr(), lp.data_ptr()
+    dev = logits.device
+    entropy = torch.empty(T, dtype=torch.float32, device=dev)
+    top = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    ids = torch.empty((T, top_k), dtype=torch.int64, device=dev)
+    held, ws_ptr, ws_bytes = _scratch(workspace, 0 if workspace is not None else _logprobs_workspace_bytes(T, V, top_k), dev)
+    code = _lib.load().m355_token_logprobs(logits.data_ptr(), logits.stride(0) if T > 1 else V, tok_ptr, given, T, V, top_k, temperature, lp_ptr,
+                                           entropy.data_ptr(), top.data_ptr(), ids.data_ptr(), ws_ptr, ws_bytes, dtype_code(logits.dtype),
+                                           current_stream())
+    if code:
+        check(code, "m355_token_logprobs")
     return TokenLogprobs(lp, entropy, top, ids)
+
+
+@functools.lru_cache(maxsize=1024)
+def _logprobs_workspace_bytes(T: int, V: int, top_k: int) -> int:
+    return int(_lib.load().m355_token_logprobs_workspace_bytes(T, V, top_k))
