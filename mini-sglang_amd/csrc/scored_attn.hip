@@ -8,8 +8,8 @@
 // drafted tokens, the prefix and the row's ancestors (tree_bits).
 //
 // A query row is a (token, q head of the group) pair, token-major, so the G heads that share a kv head share its loads.  Two
-// kernels, by the rows a request brings: scored_few_kernel (decode steps, small trees: HBM-bound) and scored_wide_kernel (long
-// extends, large trees: bound by the vector unit's exponentials and the matrix unit).  Both walk [lo_min, hi_max) of their
+// kernels, by the rows a request brings: scored_few_kernel (single tokens: HBM-bound) and scored_wide_kernel (long
+// extends, trees: bound by the vector unit's exponentials and the matrix unit, short ones by HBM).  Both walk [lo_min, hi_max) of their
 // rows only, in one pass with the running maximum and sum of the softmax, and cut that range into splits when there are too few row
 // blocks for 256 CUs; scored_merge_kernel then joins the splits.  Nothing is accumulated by atomics: results do not depend on
 // an order of arrival.
@@ -24,73 +24,67 @@
 
 namespace m355 {
 
+// the range of the rows of 16 neighbouring lanes, in all of them
+template <int CTRL>
+__device__ __forceinline__ BlockRange join_dpp(BlockRange a) {
+    const int lo = __builtin_amdgcn_update_dpp(a.lo_min, a.lo_min, CTRL, 0xF, 0xF, true), hi = __builtin_amdgcn_update_dpp(a.hi_max, a.hi_max, CTRL, 0xF, 0xF, true);
+    const int lx = __builtin_amdgcn_update_dpp(a.lo_max, a.lo_max, CTRL, 0xF, 0xF, true), hn = __builtin_amdgcn_update_dpp(a.hi_min, a.hi_min, CTRL, 0xF, 0xF, true);
+    return {imin(a.lo_min, lo), imax(a.hi_max, hi), imax(a.lo_max, lx), imin(a.hi_min, hn)};
+}
+__device__ __forceinline__ BlockRange join16(BlockRange a) {
+    return join_dpp<kDppMirror>(join_dpp<kDppHalfMirror>(join_dpp<kDppXor2>(join_dpp<kDppXor1>(a))));
+}
+
 // softmax(-inf everywhere so far): the difference of two -inf would be NaN
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
 
 // ------------------------------------------------------------------------------------------------------------------------
-// Few rows: a workgroup takes up to 16 RT rows of one (request, kv head) and one split of the keys.  Its four waves walk tiles
-// of 32 keys on their own (tile 4 i + wave), each with its own two-stage LDS ring filled by LDS-DMA, and hold all rows: K and V
-// are read from memory once per workgroup and from LDS once per wave, and no barrier sits in the loop.  The waves' results
-// meet in LDS at the end.
+// Up to 16 rows (single tokens): a workgroup takes the rows of one (request, kv head) and one split of the keys.  Its two waves
+// walk tiles of 32 keys on their own (tile 2 i + wave), each with its own two-stage LDS ring filled by LDS-DMA: K and V are read once,
+// no barrier sits in the loop, and the waves' results meet in LDS at the end.
 //   S^T[key, row]  = K[32 x D] . Q^T[D x 16]   v_mfma_f32_16x16x32: a lane owns one row and 8 of the tile's keys
 //   O^T[d, row]   += V^T[D x 32] . P^T[32 x 16]   P^T is the S^T accumulator rounded in place, V^T is read transposed
+// Bound by HBM.  Two waves: the LDS then holds two workgroups a CU at head_dim 128 and four at 64, whose starts and ends overlap
+// (16 requests of 20 000 to 32 768 tokens, 222 MB: 41.6 us, 5.3 TB/s; with four waves 49.8, with one 58.7).  More rows go to
+// the other kernel: with 32 rows here, 16 requests of 2 250 tokens took 45 us against 29.
 // ------------------------------------------------------------------------------------------------------------------------
-constexpr int kFewSlots = 2048;                       // tokens whose pool slots are in LDS at a time
+constexpr int kFewRows = 16, kFewWaves = 2;
+constexpr int kFewSlots = 1024;                       // tokens whose pool slots are in LDS at a time
 
-template <int D, int RT, bool MOD, bool F16>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void scored_few_kernel(const ScoredParams p) {
+template <int D, bool MOD, bool F16>
+__global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const ScoredParams p) {
     using M = MG<D>;
-    constexpr int RW = 16 * RT, PITCH = D + 4;
-    constexpr int RING = 8 * M::STAGEB, JOIN = 4 * RW * (PITCH + 2) * 4;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[RING > JOIN ? RING : JOIN];
+    constexpr int NW = kFewWaves, NT = 64 * NW, PITCH = D + 4;
+    constexpr int RING = 2 * NW * M::STAGEB, JOIN = NW * kFewRows * (PITCH + 2) * 4;
+    static_assert(JOIN <= RING, "the waves' results fit where the rings were");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[RING];
     __shared__ int32_t slots[kFewSlots];
     const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
 
-    // ---- which rows and keys.  Row blocks of one (request, kv head, split) follow one another on one XCD (workgroups go round
-    // the 8 XCDs), so that they share the keys in its L2; the kv head rotates with the unit so that no XCD reads one column only.
-    const int y = blockIdx.x >> 3, rb = y % p.blocks;
-    const int u = (y / p.blocks) * 8 + (blockIdx.x & 7);
-    if (u >= p.splits * p.B * p.Hkv) return;
-    const int h = (u + u / p.Hkv) % p.Hkv, b = u / p.Hkv % p.B, sp = u / (p.Hkv * p.B);
+    // ---- which rows and keys.  The kv head rotates with the unit: workgroups go round the 8 XCDs, and an XCD should not read one
+    // head's column of the pools only.
+    const int u = blockIdx.x, h = (u + u / p.Hkv) % p.Hkv, b = u / p.Hkv % p.B, sp = u / (p.Hkv * p.B);
     const ReqSpan r = load_span(p, b);
-    const int row0 = rb * RW, rows = r.E * p.G;
-    if (row0 >= rows) return;
+    const int rows = r.E * p.G;
+    if (rows == 0) return;
     const int32_t* pt_row = table_row(p, b);
-
-    // ---- the lane's rows
-    int32_t lo[RT], hi[RT], pos[RT], tr[RT], gr[RT];
-    bool ok[RT];
-    float slope[RT];
-    BlockRange br = block_range(p, r, b, row0 / p.G, imin(r.E - 1, (row0 + RW - 1) / p.G));
-    if (p.doc_starts) br = {0x7fffffff, 0, 0, 0x7fffffff};
-#pragma unroll
-    for (int x = 0; x < RT; ++x) {
-        const int m = row0 + 16 * x + n;
-        ok[x] = m < rows;
-        const int j = ok[x] ? m / p.G : 0;
-        gr[x] = ok[x] ? m - j * p.G : 0;
-        tr[x] = r.q0 + j;
-        pos[x] = r.P + j;
-        if (p.mask) {
-            lo[x] = 0; hi[x] = r.L;
-            if (MOD && p.slopes) pos[x] = (int32_t)p.positions[tr[x]];
-        } else {
-            const KeyRange v = visible_range(pos[x], r.L, p.window, p.doc_starts ? p.doc_starts[tr[x]] : 0, p.bidir ? p.bidir[b] : 0);
-            lo[x] = v.lo; hi[x] = v.hi;
-        }
-        slope[x] = MOD && p.slopes ? p.slopes[h * p.G + gr[x]] * kLog2e : 0.f;
-        if (p.doc_starts && ok[x]) {
-            if (lo[x] < hi[x]) { br.lo_min = imin(br.lo_min, lo[x]); br.hi_max = imax(br.hi_max, hi[x]); }
-            br.lo_max = imax(br.lo_max, lo[x]); br.hi_min = imin(br.hi_min, hi[x]);
-        }
+    const bool ok = n < rows;
+    const int j = ok ? n / p.G : 0, g = ok ? n - j * p.G : 0;
+    const int64_t t = r.q0 + j;
+    int32_t lo = 0, hi = r.L, pos = r.P + j;
+    BlockRange br;
+    if (p.mask) {
+        if (MOD && p.slopes) pos = (int32_t)p.positions[t];
+    } else {
+        const KeyRange v = visible_range(pos, r.L, p.window, p.doc_starts ? p.doc_starts[t] : 0, p.bidir ? p.bidir[b] : 0);
+        lo = v.lo; hi = v.hi;
     }
-    if (p.doc_starts) {
-#pragma unroll
-        for (int x = 1; x < 16; x <<= 1) {
-            br.lo_min = imin(br.lo_min, __shfl_xor(br.lo_min, x)); br.hi_max = imax(br.hi_max, __shfl_xor(br.hi_max, x));
-            br.lo_max = imax(br.lo_max, __shfl_xor(br.lo_max, x)); br.hi_min = imin(br.hi_min, __shfl_xor(br.hi_min, x));
-        }
+    if (!p.doc_starts) {
+        br = block_range(p, r, b, 0, r.E - 1);
+    } else {
+        const bool some = ok && lo < hi;
+        br = join16({some ? lo : 0x7fffffff, some ? hi : 0, ok ? lo : 0, ok ? hi : 0x7fffffff});
     }
     const int lo_min = __builtin_amdgcn_readfirstlane(br.lo_min), hi_max = __builtin_amdgcn_readfirstlane(br.hi_max);
     const int lo_max = __builtin_amdgcn_readfirstlane(br.lo_max), hi_min = __builtin_amdgcn_readfirstlane(br.hi_min);
@@ -98,25 +92,19 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void scored_few_kernel(const 
     const int active = imax(1, imin(p.splits, (keys + p.chunk - 1) / p.chunk));
     if (sp >= active) return;
     const int t0 = first + sp * p.chunk, t1 = keys ? (sp == active - 1 ? hi_max : t0 + p.chunk) : t0;
+    const float slope = MOD && p.slopes ? p.slopes[h * p.G + g] * kLog2e : 0.f;
 
-    bf16x8 qf[RT][M::KS];
+    bf16x8 qf[M::KS];
 #pragma unroll
-    for (int x = 0; x < RT; ++x)
-#pragma unroll
-        for (int s = 0; s < M::KS; ++s) {
-            u32x4 w = {0u, 0u, 0u, 0u};
-            if (ok[x]) w = *reinterpret_cast<const u32x4*>(p.q + tr[x] * p.q_stride + (int64_t)(h * p.G + gr[x]) * D + 32 * s + 8 * kg);
-            qf[x][s] = __builtin_bit_cast(bf16x8, w);
-        }
-
-    f32x4 O[RT][M::DT];
-    float m_run[RT], l_run[RT];
-#pragma unroll
-    for (int x = 0; x < RT; ++x) {
-        m_run[x] = -INFINITY; l_run[x] = 0.f;
-#pragma unroll
-        for (int dt = 0; dt < M::DT; ++dt) O[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < M::KS; ++s) {
+        u32x4 w = {0u, 0u, 0u, 0u};
+        if (ok) w = *reinterpret_cast<const u32x4*>(p.q + t * p.q_stride + (int64_t)(h * p.G + g) * D + 32 * s + 8 * kg);
+        qf[s] = __builtin_bit_cast(bf16x8, w);
     }
+    f32x4 O[M::DT];
+#pragma unroll
+    for (int dt = 0; dt < M::DT; ++dt) O[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_run = 0.f;
 
     // ---- per-lane constants of the DMA and of the LDS reads (stream_plan.h MG: chunk ch of a row sits at ch ^ s(row))
     const int drow = lane / M::C, dch = lane % M::C;
@@ -137,13 +125,13 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void scored_few_kernel(const 
 
     int w0 = t0, wn = 0;                              // the slot window: tokens w0 .. w0 + wn
     auto issue = [&](const int tile, const int st) {
-        int64_t ro[M::NI];
+        uint64_t ro[M::NI];
 #pragma unroll
-        for (int i = 0; i < M::NI; ++i) ro[i] = slots[imin(32 * tile + i * M::RPI + drow, wn - 1)];
+        for (int i = 0; i < M::NI; ++i) ro[i] = (uint64_t)(uint32_t)slots[imin(32 * tile + i * M::RPI + drow, wn - 1)] * row_bytes;
 #pragma unroll
         for (int i = 0; i < M::NI; ++i) {
-            glds16p<1>(kbase + ro[i] * row_bytes + koff[i], ring0 + st * M::STAGEB + 1024 * i);
-            glds16p<1>(vbase + ro[i] * row_bytes + voff[i], ring0 + st * M::STAGEB + M::TILEB + 1024 * i);
+            glds16p<1>(kbase + ro[i] + koff[i], ring0 + st * M::STAGEB + 1024 * i);
+            glds16p<1>(vbase + ro[i] + voff[i], ring0 + st * M::STAGEB + M::TILEB + 1024 * i);
         }
     };
     auto v_frag = [&](const uint8_t* st, const int dt) {
@@ -154,123 +142,88 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void scored_few_kernel(const 
     };
     auto consume = [&](const int base, const int stage) {
         const uint8_t* st = ring + stage * M::STAGEB;
-        f32x4 s0[RT], s1[RT];
-#pragma unroll
-        for (int x = 0; x < RT; ++x) s0[x] = s1[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < M::KS; ++s) {
             const bf16x8 a0 = *reinterpret_cast<const bf16x8*>(st + (ka0 ^ (64 * s)));
             const bf16x8 a1 = *reinterpret_cast<const bf16x8*>(st + 16 * M::ROWB + (ka0 ^ (64 * s)));
-#pragma unroll
-            for (int x = 0; x < RT; ++x) {
-                s0[x] = mfma_16x16x32<F16>(a0, qf[x][s], s0[x]);
-                s1[x] = mfma_16x16x32<F16>(a1, qf[x][s], s1[x]);
-            }
+            s0 = mfma_16x16x32<F16>(a0, qf[s], s0);
+            s1 = mfma_16x16x32<F16>(a1, qf[s], s1);
         }
-        // this lane: row n of each tile, keys base + 4 kg + i and base + 16 + 4 kg + i
+        // this lane: row n, keys base + 4 kg + i and base + 16 + 4 kg + i
+        float s[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
         if constexpr (MOD) {
             if (p.cap_log2 > 0.f) {
 #pragma unroll
-                for (int x = 0; x < RT; ++x)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { s0[x][i] = cap_score(p, s0[x][i]); s1[x][i] = cap_score(p, s1[x][i]); }
+                for (int i = 0; i < 8; ++i) s[i] = cap_score(p, s[i]);
             } else {
 #pragma unroll
-                for (int x = 0; x < RT; ++x) { s0[x] *= p.scale_log2; s1[x] *= p.scale_log2; }
+                for (int i = 0; i < 8; ++i) s[i] *= p.scale_log2;
             }
             if (p.slopes) {
                 if (p.mask && base + 32 > r.P) {          // some keys are nodes: their positions are their depths
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int tok = base + 16 * (i >> 2) + 4 * kg + (i & 3);
-                        const int node = imin(imax(tok - r.P, 0), r.E - 1);
-                        const int kp = tok < r.P ? tok : (int)p.positions[r.q0 + node];
-#pragma unroll
-                        for (int x = 0; x < RT; ++x) {
-                            const float away = fabsf((float)(pos[x] - kp));
-                            if (i < 4) s0[x][i & 3] = fmaf(-slope[x], away, s0[x][i & 3]);
-                            else s1[x][i & 3] = fmaf(-slope[x], away, s1[x][i & 3]);
-                        }
+                        const int kp = tok < r.P ? tok : (int)p.positions[r.q0 + imin(tok - r.P, r.E - 1)];
+                        s[i] = fmaf(-slope, fabsf((float)(pos - kp)), s[i]);
                     }
                 } else {
+                    const float d = (float)(pos - base - 4 * kg);
 #pragma unroll
-                    for (int x = 0; x < RT; ++x) {
-                        const float d = (float)(pos[x] - base - 4 * kg);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            s0[x][i] = fmaf(-slope[x], fabsf(d - (float)i), s0[x][i]);
-                            s1[x][i] = fmaf(-slope[x], fabsf(d - (float)(16 + i)), s1[x][i]);
-                        }
-                    }
+                    for (int i = 0; i < 8; ++i) s[i] = fmaf(-slope, fabsf(d - (float)(16 * (i >> 2) + (i & 3))), s[i]);
                 }
             }
         }
         const bool part = base < lo_max || base + 32 > hi_min;             // wave-uniform
-        uint32_t bits[RT];
+        uint32_t bits = 0;
         bool bad = false;
         if (part) {
+            bits = row_bits(p, r, t, lo, hi, base);
+            const uint32_t w = bits >> (4 * kg);
 #pragma unroll
-            for (int x = 0; x < RT; ++x) {
-                bits[x] = row_bits(p, r, tr[x], lo[x], hi[x], base);
-                const uint32_t w = bits[x] >> (4 * kg);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s0[x][i] = (w >> i) & 1u ? s0[x][i] : -INFINITY;
-                    s1[x][i] = (w >> (16 + i)) & 1u ? s1[x][i] : -INFINITY;
-                }
-            }
+            for (int i = 0; i < 8; ++i) s[i] = (w >> (16 * (i >> 2) + (i & 3))) & 1u ? s[i] : -INFINITY;
             bool any = false;
 #pragma unroll
             for (int dt = 0; dt < M::DT; ++dt) any = any || frag_nonfinite<F16>(v_frag(st, dt));
             bad = __any(any);
         }
-        bf16x8 pf[RT];
+        float mx = s[0], a, c;
 #pragma unroll
-        for (int x = 0; x < RT; ++x) {
-            float mx = fmaxf(fmaxf(fmaxf(s0[x][0], s0[x][1]), fmaxf(s0[x][2], s0[x][3])), fmaxf(fmaxf(s1[x][0], s1[x][1]), fmaxf(s1[x][2], s1[x][3])));
-            float a, c;
-            lane_pair<16>(mx, a, c);
-            mx = fmaxf(a, c);
-            lane_pair<32>(mx, a, c);
-            mx = fmaxf(a, c);
-            if constexpr (!MOD) mx *= p.scale_log2;
-            // the running maximum moves only when beaten by 2^kLazyMax: rescaling is rare, weights stay below 2^kLazyMax
-            const float m_new = mx > m_run[x] + kLazyMax ? mx : m_run[x];
-            const float alpha = m_new == m_run[x] ? 1.f : exp2_fast(m_run[x] - m_new);
-            m_run[x] = m_new;
-            const float mu = finite_max(m_new);
-            float sum = 0.f;
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
+        lane_pair<16>(mx, a, c);
+        mx = fmaxf(a, c);
+        lane_pair<32>(mx, a, c);
+        mx = fmaxf(a, c);
+        if constexpr (!MOD) mx *= p.scale_log2;
+        // the running maximum moves only when beaten by 2^kLazyMax: rescaling is rare, weights stay below 2^kLazyMax
+        const float m_new = mx > m_run + kLazyMax ? mx : m_run;
+        const float alpha = m_new == m_run ? 1.f : exp2_fast(m_run - m_new);
+        m_run = m_new;
+        const float mu = finite_max(m_new);
+        float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s0[x][i] = exp2_fast(MOD ? s0[x][i] - mu : fmaf(s0[x][i], p.scale_log2, -mu));
-                s1[x][i] = exp2_fast(MOD ? s1[x][i] - mu : fmaf(s1[x][i], p.scale_log2, -mu));
-                sum += s0[x][i] + s1[x][i];
-            }
-            l_run[x] = fmaf(l_run[x], alpha, sum);
-            if (__any(alpha != 1.f)) {
+        for (int i = 0; i < 8; ++i) { s[i] = exp2_fast(MOD ? s[i] - mu : fmaf(s[i], p.scale_log2, -mu)); sum += s[i]; }
+        l_run = fmaf(l_run, alpha, sum);
+        if (__any(alpha != 1.f)) {
 #pragma unroll
-                for (int dt = 0; dt < M::DT; ++dt) O[x][dt] *= alpha;
-            }
-            pf[x] = __builtin_bit_cast(bf16x8, u32x4{pack16<F16>(s0[x][0], s0[x][1]), pack16<F16>(s0[x][2], s0[x][3]),
-                                                     pack16<F16>(s1[x][0], s1[x][1]), pack16<F16>(s1[x][2], s1[x][3])});
+            for (int dt = 0; dt < M::DT; ++dt) O[dt] *= alpha;
         }
+        // the weights go into the second product rounded to the element type, as the matrix unit takes them; their sum does not
+        const bf16x8 pf = __builtin_bit_cast(bf16x8, u32x4{pack16<F16>(s[0], s[1]), pack16<F16>(s[2], s[3]), pack16<F16>(s[4], s[5]), pack16<F16>(s[6], s[7])});
 #pragma unroll
         for (int dt = 0; dt < M::DT; ++dt) {
             bf16x8 av = v_frag(st, dt);
             if (bad) av = frag_finite<F16>(av);
-#pragma unroll
-            for (int x = 0; x < RT; ++x) O[x][dt] = mfma_16x16x32<F16>(av, pf[x], O[x][dt]);
+            O[dt] = mfma_16x16x32<F16>(av, pf, O[dt]);
         }
         if (bad) {                                                         // rare: infinities and NaN, for the rows that see them
             for (int tk = 0; tk < 32; ++tk) {
+                if (!((bits >> tk) & 1u)) continue;
                 const uint8_t* vr = st + M::TILEB + tk * M::ROWB + 8 * (kg & 1);
 #pragma unroll
-                for (int dt = 0; dt < M::DT; ++dt) {
-                    const f32x4 e = nonfinite4<F16>(*reinterpret_cast<const uint2*>(vr + 16 * ((2 * dt + (kg >> 1)) ^ M::sV(tk))));
-#pragma unroll
-                    for (int x = 0; x < RT; ++x)
-                        if ((bits[x] >> tk) & 1u) O[x][dt] += e;
-                }
+                for (int dt = 0; dt < M::DT; ++dt)
+                    O[dt] += nonfinite4<F16>(*reinterpret_cast<const uint2*>(vr + 16 * ((2 * dt + (kg >> 1)) ^ M::sV(tk))));
             }
         }
     };
@@ -278,64 +231,59 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void scored_few_kernel(const 
     for (; w0 < t1; w0 += kFewSlots) {
         wn = imin(kFewSlots, t1 - w0);
         __syncthreads();
-        for (int i = threadIdx.x; i < wn; i += 256) slots[i] = slot_of(p, pt_row, w0 + i);
+        for (int i = threadIdx.x; i < wn; i += NT) slots[i] = slot_of(p, pt_row, w0 + i);
         __syncthreads();
         const int nt = (wn + 31) >> 5;
         if (wid < nt) issue(wid, 0);
-        for (int t = wid; t < nt; t += 8) {
-            if (t + 4 < nt) { issue(t + 4, 1); wait_vmcnt<2 * M::NI>(); } else wait_vmcnt<0>();
-            consume(w0 + 32 * t, 0);
-            if (t + 4 >= nt) break;
-            if (t + 8 < nt) { issue(t + 8, 0); wait_vmcnt<2 * M::NI>(); } else wait_vmcnt<0>();
-            consume(w0 + 32 * (t + 4), 1);
+        for (int k = wid; k < nt; k += 2 * NW) {
+            if (k + NW < nt) { issue(k + NW, 1); wait_vmcnt<2 * M::NI>(); } else wait_vmcnt<0>();
+            consume(w0 + 32 * k, 0);
+            if (k + NW >= nt) break;
+            if (k + 2 * NW < nt) { issue(k + 2 * NW, 0); wait_vmcnt<2 * M::NI>(); } else wait_vmcnt<0>();
+            consume(w0 + 32 * (k + NW), 1);
         }
     }
 
-    // ---- the four waves' results meet in LDS
+    // ---- the waves' results meet in LDS
     float* const jo = reinterpret_cast<float*>(smem);
-    float* const jm = jo + 4 * RW * PITCH;                                  // (m, l) per wave and row
+    float* const jm = jo + NW * kFewRows * PITCH;                           // (m, l) per wave and row
+    float a, c;
+    lane_pair<16>(l_run, a, c);
+    float l_sum = a + c;
+    lane_pair<32>(l_sum, a, c);
+    l_sum = a + c;
     __syncthreads();
+    if (kg == 0) *reinterpret_cast<float2*>(jm + 2 * (wid * kFewRows + n)) = make_float2(m_run, l_sum);
 #pragma unroll
-    for (int x = 0; x < RT; ++x) {
-        float a, c;
-        lane_pair<16>(l_run[x], a, c);
-        float l = a + c;
-        lane_pair<32>(l, a, c);
-        l = a + c;
-        const int row = wid * RW + 16 * x + n;
-        if (kg == 0) *reinterpret_cast<float2*>(jm + 2 * row) = make_float2(m_run[x], l);
-#pragma unroll
-        for (int dt = 0; dt < M::DT; ++dt) *reinterpret_cast<f32x4*>(jo + row * PITCH + 16 * dt + 4 * kg) = O[x][dt];
-    }
+    for (int dt = 0; dt < M::DT; ++dt) *reinterpret_cast<f32x4*>(jo + (wid * kFewRows + n) * PITCH + 16 * dt + 4 * kg) = O[dt];
     __syncthreads();
     constexpr int CH = D / 4;
-    for (int i = threadIdx.x; i < RW * CH; i += 256) {
-        const int row = i / CH, c = i % CH, m = row0 + row;
-        if (m >= rows) break;
-        float mw[4], mx = -INFINITY, l = 0.f;
+    for (int i = threadIdx.x; i < rows * CH; i += NT) {
+        const int m = i / CH, ch = i % CH;
+        float mw[NW], mx = -INFINITY, l = 0.f;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) { mw[w] = jm[2 * (w * RW + row)]; mx = fmaxf(mx, mw[w]); }
+        for (int w = 0; w < NW; ++w) { mw[w] = jm[2 * (w * kFewRows + m)]; mx = fmaxf(mx, mw[w]); }
         const float mu = finite_max(mx);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float e = exp2_fast(mw[w] - mu);
-            l = fmaf(e, jm[2 * (w * RW + row) + 1], l);
-            o += *reinterpret_cast<const f32x4*>(jo + (w * RW + row) * PITCH + 4 * c) * e;
+            l = fmaf(e, jm[2 * (w * kFewRows + m) + 1], l);
+            o += *reinterpret_cast<const f32x4*>(jo + (w * kFewRows + m) * PITCH + 4 * ch) * e;
         }
-        const int j = m / p.G, head = h * p.G + m - j * p.G;
-        const int64_t item = (int64_t)(r.q0 + j) * p.Hq + head;
+        const int row = m / p.G, head = h * p.G + m - row * p.G;
+        const int64_t item = (int64_t)(r.q0 + row) * p.Hq + head;
         if (active > 1) {
             float* wo = p.part + (item * p.splits + sp) * (D + 4);
-            *reinterpret_cast<f32x4*>(wo + 4 * c) = o;
-            if (c == 0) *reinterpret_cast<float2*>(wo + D) = make_float2(mx, l);
+            *reinterpret_cast<f32x4*>(wo + 4 * ch) = o;
+            if (ch == 0) *reinterpret_cast<float2*>(wo + D) = make_float2(mx, l);
         } else {
             const float inv = 1.f / l;
             uint2 w = {0u, 0u};
             if (l != 0.f) w = make_uint2(pack16<F16>(o[0] * inv, o[1] * inv), pack16<F16>(o[2] * inv, o[3] * inv));
-            *reinterpret_cast<uint2*>(p.out + (int64_t)(r.q0 + j) * p.o_stride + (int64_t)head * D + 4 * c) = w;
+            *reinterpret_cast<uint2*>(p.out + (int64_t)(r.q0 + row) * p.o_stride + (int64_t)head * D + 4 * ch) = w;
         }
-        if (sp == 0 && c == 0 && p.splits > 1) p.part_n[item] = active;
+        if (sp == 0 && ch == 0 && p.splits > 1) p.part_n[item] = active;
     }
 }
 
@@ -348,7 +296,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void scored_few_kernel(const 
 template <int D, bool MOD, bool F16>
 __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams p) {
     using W = WgCfg<D>;
-    constexpr int NW = 4, NBUF = 4, ROWS = 32 * NW, IPW = 2 * W::NI / NW, HP = IPW / 2;
+    constexpr int NW = 4, NBUF = 4;
+    constexpr int NT = 64 * NW, ROWS = 32 * NW, IPW = 2 * W::NI / NW, HP = IPW / 2;
+    constexpr int NP = NBUF / 2;                      // pairs the ring holds: NP - 1 are on their way while one is worked on
+    static_assert(IPW % 2 == 0 && W::NI % NW == 0 && NP == 2 && NBUF * W::TILEB <= 65536, "ring geometry");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[NBUF * W::BUFB];      // NBUF K tiles, NBUF V tiles
     __shared__ int32_t slotw[kSlotWin];
     __shared__ int32_t wlim[NW][2];
@@ -392,14 +343,12 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
             if (lo < hi) { br.lo_min = lo; br.hi_max = hi; }
             br.lo_max = lo; br.hi_min = hi;
         }
-#pragma unroll
-        for (int x = 1; x < 32; x <<= 1) {
-            br.lo_min = imin(br.lo_min, __shfl_xor(br.lo_min, x)); br.hi_max = imax(br.hi_max, __shfl_xor(br.hi_max, x));
-            br.lo_max = imax(br.lo_max, __shfl_xor(br.lo_max, x)); br.hi_min = imin(br.hi_min, __shfl_xor(br.hi_min, x));
-        }
+        br = join16(br);
+        br.lo_min = imin(br.lo_min, __shfl_xor(br.lo_min, 16)); br.hi_max = imax(br.hi_max, __shfl_xor(br.hi_max, 16));
+        br.lo_max = imax(br.lo_max, __shfl_xor(br.lo_max, 16)); br.hi_min = imin(br.hi_min, __shfl_xor(br.hi_min, 16));
     }
     if (br.lo_min >= br.hi_max) { br.lo_min = 0x7fffffff; br.hi_max = 0; }
-    if (l == 0) { wlim[wid][0] = br.lo_min; wlim[wid][1] = br.hi_max; }
+    if (p.doc_starts && l == 0) { wlim[wid][0] = br.lo_min; wlim[wid][1] = br.hi_max; }
     const int w_lo_min = __builtin_amdgcn_readfirstlane(br.lo_min), w_hi_max = __builtin_amdgcn_readfirstlane(br.hi_max);
     const int w_lo_max = __builtin_amdgcn_readfirstlane(br.lo_max), w_hi_min = __builtin_amdgcn_readfirstlane(br.hi_min);
 
@@ -419,10 +368,16 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
             for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
     }
     const float slope = MOD && p.slopes ? p.slopes[h * p.G + g] * kLog2e : 0.f;
-    __syncthreads();
-    int lo_wg = wlim[0][0], hi_wg = wlim[0][1];
+    int lo_wg, hi_wg;
+    if (p.doc_starts) {
+        __syncthreads();
+        lo_wg = wlim[0][0]; hi_wg = wlim[0][1];
 #pragma unroll
-    for (int x = 1; x < NW; ++x) { lo_wg = imin(lo_wg, wlim[x][0]); hi_wg = imax(hi_wg, wlim[x][1]); }
+        for (int x = 1; x < NW; ++x) { lo_wg = imin(lo_wg, wlim[x][0]); hi_wg = imax(hi_wg, wlim[x][1]); }
+    } else {                                                       // (no barrier, and no wait for the q fragments, where the rows' ends tell)
+        const BlockRange w = block_range(p, r, b, ROWS * tb / p.G, imin(r.E - 1, (ROWS * tb + ROWS - 1) / p.G));
+        lo_wg = w.lo_min; hi_wg = w.hi_max;
+    }
     lo_wg = __builtin_amdgcn_readfirstlane(lo_wg); hi_wg = __builtin_amdgcn_readfirstlane(hi_wg);
     const bool none = lo_wg >= hi_wg;
     const int pair0 = none ? 0 : lo_wg >> 6, pairs_end = none ? 0 : (hi_wg + 63) >> 6, n_tiles = (hi_wg + 31) >> 5;
@@ -441,8 +396,8 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     auto fill_slots = [&](int win) {
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kSlotWin / 256; ++k) {
-            const int i = (int)threadIdx.x + 256 * k;
+        for (int k = 0; k < kSlotWin / NT; ++k) {
+            const int i = (int)threadIdx.x + NT * k;
             slotw[i] = slot_of(p, pt_row, imin(win * kSlotWin + i, hi_wg - 1));
         }
         __syncthreads();
@@ -582,13 +537,13 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     };
 
     auto pair_step = [&](const int k, auto pb_const) {
-        constexpr int pb = decltype(pb_const)::value, nb = 2 * (1 - pb);
-        wait_vmcnt<0>();                                           // pair k has landed
+        constexpr int pb = decltype(pb_const)::value, nb = 2 * ((pb + NP - 1) % NP);
+        wait_vmcnt<(NP - 2) * 2 * IPW>();                          // pair k has landed; NP - 2 younger pairs stay in flight
         __syncthreads();                                           // ... everybody's part of it, and everyone left pair k - 1
         int32_t sl[IPW];
         const int base_a = 64 * k, base_b = 64 * k + 32;
         if (base_a >= w_hi_max || base_a + 64 <= w_lo_min) {       // wave-uniform: nothing here for this wave's rows
-            pair_slots(k + 1, sl);
+            pair_slots(k + NP - 1, sl);
 #pragma unroll
             for (int x = 0; x < IPW; ++x) { piece(false, x, sl[x], nb); piece(true, x, sl[x], nb); }
             return;
@@ -597,7 +552,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
         f32x16 sa, sb;
 #pragma unroll
         for (int s = 0; s < W::KS; ++s) fa[s] = rdk(2 * pb, s);
-        pair_slots(k + 1, sl);
+        pair_slots(k + NP - 1, sl);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 16; ++i) { sa[i] = 0.f; sb[i] = 0.f; }
@@ -650,11 +605,15 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     };
     if (!none) {
         fill_slots((2 * p_begin) / (kSlotWin / 32));
-        int32_t sl[IPW];
-        pair_slots(p_begin, sl);
+        wait_vmcnt<0>();                                           // q fragments are in: the DMA count starts clean
 #pragma unroll
-        for (int x = 0; x < IPW; ++x) { piece(false, x, sl[x], 0); piece(true, x, sl[x], 0); }
-        for (int k0 = p_begin; k0 < n_pairs; k0 += 2) {
+        for (int y = 0; y < NP - 1; ++y) {
+            int32_t sl[IPW];
+            pair_slots(p_begin + y, sl);
+#pragma unroll
+            for (int x = 0; x < IPW; ++x) { piece(false, x, sl[x], 2 * y); piece(true, x, sl[x], 2 * y); }
+        }
+        for (int k0 = p_begin; k0 < n_pairs; k0 += NP) {
             pair_step(k0, IntC<0>{});
             if (k0 + 1 < n_pairs) pair_step(k0 + 1, IntC<1>{});
         }
@@ -701,33 +660,39 @@ __global__ __launch_bounds__(256) void scored_merge_kernel(const ScoredParams p)
     const int64_t row = item / p.Hq, head = item - row * p.Hq;
     const int64_t r0 = p.cu_q ? imax(p.cu_q[0], 0) : 0, r1 = p.cu_q ? imin(p.cu_q[p.B], p.T) : imin(p.B, p.T);
     if (row < r0 || row >= r1) return;                              // rows of no request: left as they were
-    const int n = imin(p.part_n[item], p.splits);
-    if (n <= 1) return;                                             // written by the attention kernel
+    // The first eight parts are requested together with their number: parts that nobody wrote are left out by selection, never
+    // by a factor.
     const float* base = p.part + item * p.splits * (D + 4);
+    const int held = p.part_n[item];
     float mx = -INFINITY, den = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    int n = p.splits;
     for (int s0 = 0; s0 < n; s0 += CH) {
-        float m[CH], l[CH];
+        float2 ml[CH];
         f32x4 o[CH];
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
             const float* ps = base + (int64_t)imin(s0 + k, n - 1) * (D + 4);
-            const float2 ml = *reinterpret_cast<const float2*>(ps + D);
-            m[k] = s0 + k < n ? ml.x : -INFINITY;
-            l[k] = s0 + k < n ? ml.y : 0.f;
+            ml[k] = *reinterpret_cast<const float2*>(ps + D);
             o[k] = *reinterpret_cast<const f32x4*>(ps + 4 * li);
-            if (s0 + k >= n) o[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        if (s0 == 0) {
+            n = imin(held, p.splits);
+            if (n <= 1) return;                                     // written by the attention kernel
         }
         float mn = mx;
 #pragma unroll
-        for (int k = 0; k < CH; ++k) mn = fmaxf(mn, m[k]);
+        for (int k = 0; k < CH; ++k) {
+            if (s0 + k >= n) { ml[k] = make_float2(-INFINITY, 0.f); o[k] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+            mn = fmaxf(mn, ml[k].x);
+        }
         const float mu = finite_max(mn), rs = exp2_fast(mx - mu);
         den *= rs;
         acc *= rs;
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
-            const float w = exp2_fast(m[k] - mu);
-            den = fmaf(w, l[k], den);
+            const float w = exp2_fast(ml[k].x - mu);
+            den = fmaf(w, ml[k].y, den);
             acc += o[k] * w;
         }
         mx = mn;
@@ -749,28 +714,33 @@ static int shift_of(int32_t x) {
 }
 
 // How a call is cut, from its sizes alone (so that the workspace query and the launch agree).
-struct ScoredCut { bool wide; int rt; int32_t blocks, splits, chunk; int64_t part_bytes, bytes; };
+//
+// The rows a request brings choose the kernel.  Keys are split where there are fewer (request, kv head, row block) units than
+// workgroups the chip holds at once: two a CU (four of the small ones at head_dim 64).  One round of equal splits is what
+// pays: more, shorter ones cost a start of ~5 us each and parts to join (16 trees of 32 nodes over 2 250 tokens: 4 splits 38.2 +
+// 8.7 us, 8 splits 50.8 + 12.7, none 58.1).  A split is at least 256 keys, or a sixteenth of the range where that is shorter - a
+// single short request is a matter of latency (8 nodes over 700 tokens: 64 keys 9.8 + 4.2 us, 128 keys 13.4 + 3.5, 256 keys
+// 15.6 + 3.8; over 4 250 tokens: 256 keys 12.3 + 4.8, 128 keys 11.8 + 6.3).
+struct ScoredCut { bool wide; int32_t blocks, splits, chunk; int64_t part_bytes, bytes; };
 static ScoredCut scored_cut(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int32_t D, int64_t ext, int64_t max_len, int64_t window) {
     ScoredCut c = {};
     const int64_t G = Hq / Hkv;
     if (ext > T) ext = T;
-    const int64_t rows = ext * G;
-    c.wide = rows > 64;
-    c.rt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
-    const int64_t per_block = c.wide ? 128 : 16 * c.rt;
+    const int64_t rows = ext * G, per_block = rows > kFewRows ? 128 : kFewRows;
+    c.wide = rows > kFewRows;
     c.blocks = (int32_t)((rows + per_block - 1) / per_block);
     int64_t span = window > 0 && window + ext < max_len ? window + ext : max_len;
-    span += c.wide ? 63 : 31;                                       // the first tile may begin before the first visible key
-    // workgroups there are without splits (a ragged batch has fewer row blocks than its longest request suggests)
+    span += 63;                                                     // the first tile may begin before the first visible key
+    // (a ragged batch has fewer row blocks than its longest request suggests)
     int64_t units = B * Hkv * c.blocks;
     const int64_t packed = Hkv * ((T * G + per_block - 1) / per_block + B);
     if (packed < units) units = packed;
-    const int64_t target = c.wide || D == 128 ? 512 : 1024, shortest = c.wide ? 512 : 128;
-    int64_t splits = target / units;
+    int64_t splits = (c.wide || D == 128 ? 512 : 1024) / units;
     if (splits < 1) splits = 1;
+    int64_t shortest = span / 16;
+    if (shortest > 256) shortest = 256;
     int64_t chunk = (span + splits - 1) / splits;
     if (chunk < shortest) chunk = shortest;
-    if (!c.wide && chunk > kFewSlots) chunk = kFewSlots;
     chunk = (chunk + 63) / 64 * 64;
     splits = (span + chunk - 1) / chunk;
     c.splits = (int32_t)splits;
@@ -802,11 +772,7 @@ static void launch_kernels(const ScoredParams& p, const ScoredCut& c, hipStream_
     if (c.wide) {
         hipLaunchKernelGGL((scored_wide_kernel<D, MOD, F16>), dim3((unsigned)(p.B * p.Hkv * p.blocks), (unsigned)p.splits), dim3(256), 0, st, p);
     } else {
-        const int64_t units = (int64_t)p.splits * p.B * p.Hkv;
-        const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.blocks));
-        if (c.rt == 1) hipLaunchKernelGGL((scored_few_kernel<D, 1, MOD, F16>), grid, dim3(256), 0, st, p);
-        else if (c.rt == 2) hipLaunchKernelGGL((scored_few_kernel<D, 2, MOD, F16>), grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((scored_few_kernel<D, 4, MOD, F16>), grid, dim3(256), 0, st, p);
+        hipLaunchKernelGGL((scored_few_kernel<D, MOD, F16>), dim3((unsigned)((int64_t)p.splits * p.B * p.Hkv)), dim3(64 * kFewWaves), 0, st, p);
     }
     if (p.splits > 1) {
         const int64_t lanes = (int64_t)p.T * p.Hq * (D / 4);
@@ -819,7 +785,7 @@ static int launch_scored(ScoredParams& p, int32_t max_extend_len, int32_t max_se
     if (const int e = check_common(p, max_extend_len, max_seq_len, D, scale, cap, dtype)) return e;
     const ScoredCut c = scored_cut(p.B, p.T, p.Hq, p.Hkv, D, max_extend_len, max_seq_len, p.window);
     if (c.bytes && (!workspace || workspace_bytes < c.bytes || ((uintptr_t)workspace & 255))) return M355_ERR_WORKSPACE;
-    if ((int64_t)p.B * p.Hkv * c.blocks * (c.wide ? 1 : c.splits) > 0x3fffffffLL || c.splits > 65535 ||
+    if ((int64_t)p.B * p.Hkv * c.blocks * c.splits > 0x3fffffffLL || c.splits > 65535 ||
         (int64_t)p.T * p.Hq * (D / 4) / 256 > 0x3fffffffLL) return M355_ERR_INVALID_ARG;
     p.G = p.Hq / p.Hkv; p.ps_shift = shift_of(p.ps);
     p.scale_log2 = scale * kLog2e; p.cap_log2 = cap * kLog2e; p.cap_rate = cap > 0.f ? 2.f * scale * kLog2e / cap : 0.f;
