@@ -38,6 +38,7 @@ if HERE not in sys.path:
 
 import mi355_attn as m  # noqa: E402
 from harness.llama_shell import SHAPES, HarnessRunner  # noqa: E402
+from harness.speculate import speculative_decode  # noqa: E402
 
 
 @dataclasses.dataclass
@@ -52,6 +53,8 @@ class BenchArgs:                                    # bench_one_batch.py:72-84
     model: str = "llama-3-8b"
     page_size: int = 16
     graph: bool = False                             # decode steps replayed from one captured HIP graph (GraphedDecode)
+    top_logprobs: int = 0                           # latency mode: log probabilities and alternatives of every sampled token
+    speculate: int = 0                              # decode by verifying draft trees of up to this many nodes
     fused_row_parallel: bool = False                # TP: o_proj / down_proj + all-reduce as one launch where it applies
 
     @staticmethod
@@ -66,6 +69,10 @@ class BenchArgs:                                    # bench_one_batch.py:72-84
         p.add_argument("--model", type=str, default=BenchArgs.model, choices=sorted(SHAPES))
         p.add_argument("--page-size", type=int, default=BenchArgs.page_size)
         p.add_argument("--graph", action="store_true", help="decode through one captured HIP graph per run")
+        p.add_argument("--top-logprobs", type=int, default=BenchArgs.top_logprobs,
+                       help="after every sampled token: its log probability, the entropy and this many alternatives (m355_token_logprobs)")
+        p.add_argument("--speculate", type=int, default=BenchArgs.speculate, metavar="NODES",
+                       help="decode by verifying trees of up to NODES tokens drafted from the request's history (m355_tree_attn)")
         p.add_argument("--fused-row-parallel", action="store_true",
                        help="under TP: row-parallel GEMM + all-reduce in one launch (m355_oproj_allreduce) for decode-size inputs")
 
@@ -123,7 +130,7 @@ class GraphedDecode:
         batch.mode = m.Mode.DECODE
         batch.input_ids, batch.output_ids = self.ids, None
         batch.seq_lens, batch.positions, batch.out_cache_loc = self.seq_lens, self.pos, self.loc
-        batch.cu_q = batch.row_of_token = None
+        batch.cu_q = batch.row_of_token = batch.doc_starts = batch.bidir_lens = None
         runner.attn_backend.decode_capacity_hint = sum(batch._lens_host()) + B * (n_steps + 1)
         self.taken = 0
         # step 1 eagerly on a side stream (allocator pools, workspaces, plan buffer, library handles) ...
@@ -250,6 +257,14 @@ def correctness_test(runner, bench_args: BenchArgs, rank_print):
     rank_print(f"greedy tokens agree: {100 * same:.1f}%")
     for i in range(min(B, 3)):
         rank_print(f"========== Prompt {i} ========== {ids3[i].tolist()}")
+    if bench_args.speculate:
+        reset_pools(runner)
+        first, _, batch = extend(make_reqs(prompts), runner)
+        toks, lps, steps = speculative_decode(runner, first, batch, bench_args.output_len[0] - 1, bench_args.speculate)
+        idss = torch.cat([first.unsqueeze(1).cpu(), torch.tensor(toks, dtype=torch.int64).view(B, -1)], dim=1)
+        rank_print(f"speculative decode: {steps} steps for {bench_args.output_len[0] - 1} tokens, mean log probability "
+                   f"{statistics.fmean(x for r in lps for x in r) if lps[0] else 0.0:.3f}, "
+                   f"tokens agree with the plain loop: {100 * float((idss == ids1.cpu()).float().mean()):.1f}%")
     if bench_args.graph:
         reset_pools(runner)
         _, idsg = three_phase(runner, prompts, bench_args.cut_len, bench_args.output_len[0], graph=True)
@@ -281,8 +296,15 @@ def latency_test(runner, bench_args: BenchArgs, bs: int, il: int, ol: int, rank_
         next_ids, _, batch = extend(reqs, runner)
         sync()
         prefill = time.perf_counter() - t0
-        steps = []
-        if bench_args.graph and ol > 3:
+        steps, spec_steps = [], None
+        if bench_args.speculate and ol > 1:
+            setup = None
+            t0 = time.perf_counter()
+            _, _, spec_steps = speculative_decode(runner, next_ids, batch, ol - 1, bench_args.speculate)
+            sync()
+            total_decode = time.perf_counter() - t0
+            steps = [total_decode / spec_steps] * spec_steps
+        elif bench_args.graph and ol > 3:
             t0 = time.perf_counter()
             g = GraphedDecode(next_ids, batch, runner, ol - 1)       # runs steps 1 and 2 (eager warm-up, capture + replay)
             sync()
@@ -298,7 +320,9 @@ def latency_test(runner, bench_args: BenchArgs, bs: int, il: int, ol: int, rank_
             setup = None
             for _ in range(ol - 1):
                 t0 = time.perf_counter()
-                next_ids, _ = decode(next_ids, batch, runner)
+                next_ids, logits = decode(next_ids, batch, runner)
+                if bench_args.top_logprobs:
+                    m.ops.token_logprobs(logits, next_ids, top_k=bench_args.top_logprobs)
                 sync()
                 steps.append(time.perf_counter() - t0)
             total_decode = sum(steps)
@@ -307,11 +331,12 @@ def latency_test(runner, bench_args: BenchArgs, bs: int, il: int, ol: int, rank_
             "batch_size": bs, "input_len": il, "output_len": ol, "weights": "synthetic", "dtype": "bf16",
             "prefill_latency": prefill, "prefill_throughput": bs * il / prefill,
             "median_decode_latency": statistics.median(steps) if steps else None,
-            "median_decode_throughput": bs / statistics.median(steps) if steps else None,
+            "median_decode_throughput": bs / statistics.median(steps) if steps and spec_steps is None else None,
             "total_decode_latency": total_decode,
             "decode_throughput": bs * (ol - 1) / total_decode if steps else None,
             "total_latency": prefill + total_decode, "overall_throughput": bs * (il + ol) / (prefill + total_decode),
-            "decode_graph": bool(setup is not None), "graph_setup_latency": setup,
+            "decode_graph": bool(setup is not None), "graph_setup_latency": setup, "top_logprobs": bench_args.top_logprobs,
+            "speculative_steps": spec_steps,
         }
     reset_pools(runner)
     rank_print(json.dumps(result))
@@ -338,7 +363,7 @@ def main():
             dist.init_process_group("nccl", device_id=torch.device(dev))
     rank_print = print if rank == 0 else (lambda *x, **k: None)
     shape = SHAPES[ba.model]
-    max_bs, max_len = max(ba.batch_size), max(ba.input_len) + max(ba.output_len) + ba.page_size
+    max_bs, max_len = max(ba.batch_size), max(ba.input_len) + max(ba.output_len) + ba.speculate + ba.page_size
     runner = HarnessRunner(shape, ba.page_size, max_total_tokens=max_bs * (max_len + ba.page_size) + 64 * ba.page_size,
                            max_reqs=max_bs, context_len=max_len, tp_rank=rank, tp_size=world, device=dev,
                            fused_row_parallel=ba.fused_row_parallel)

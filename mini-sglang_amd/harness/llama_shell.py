@@ -38,6 +38,9 @@ class ModelShape:
     max_position: int = 8192
     rms_eps: float = 1e-5
     tie_embeddings: bool = False
+    logit_cap: float = 0.0                # attention scores capped by a tanh
+    window: int = 0                       # keys a token sees, its own included (0: all)
+    distance_bias: bool = False           # scores biased by distance, one slope per head
 
 
 _LLAMA3_SCALING = {"rope_type": "llama3", "factor": 32.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
@@ -49,8 +52,15 @@ SHAPES = {
     "llama-3-8b": ModelShape("Llama-3-8B", 32, 4096, 14336, 32, 8, 128, 128256),
     "llama-3-70b": ModelShape("Llama-3-70B", 80, 8192, 28672, 64, 8, 128, 128256),
     "tiny": ModelShape("tiny", 2, 256, 512, 4, 2, 64, 512, max_position=2048),
+    "tiny-capped": ModelShape("tiny-capped", 2, 256, 512, 4, 2, 64, 512, max_position=2048, logit_cap=20.0, distance_bias=True),
+    "tiny-window": ModelShape("tiny-window", 2, 256, 512, 6, 2, 64, 512, max_position=2048, logit_cap=30.0, window=24),
     "tiny128": ModelShape("tiny128", 2, 512, 1024, 4, 1, 128, 512, rope_scaling=_LLAMA3_SCALING, max_position=16384),
 }
+
+
+def distance_slopes(total_heads: int, device) -> torch.Tensor:
+    """One slope per query head, a geometric sequence down from 2^(-8 / heads) to 2^-8 (fp32)."""
+    return torch.tensor([2.0 ** (-8.0 * (i + 1) / total_heads) for i in range(total_heads)], dtype=torch.float32, device=device)
 
 
 class SyntheticLlama:
@@ -89,7 +99,10 @@ class SyntheticLlama:
             del wq, wk, wv, wo, wg, wu, wd
         self.norm = torch.ones(H, device=device, dtype=dtype)
         self.rope = RotaryEmbedding(D, D, max_position or shape.max_position, shape.rope_theta, shape.rope_scaling, device)
-        self.attn = [m.Attention(i, self.heads.num_heads, self.heads.num_kv_heads, D) for i in range(shape.layers)]
+        lo = self.heads.q_head_start
+        slopes = distance_slopes(shape.heads, device)[lo:lo + self.heads.num_heads].contiguous() if shape.distance_bias else None
+        self.attn = [m.Attention(i, self.heads.num_heads, self.heads.num_kv_heads, D, logit_cap=shape.logit_cap, window=shape.window, slopes=slopes)
+                     for i in range(shape.layers)]
 
     def _norm(self, x, residual, weight):
         # RMSNorm with fused residual add (layers/layernorm.py:14-41)
@@ -107,7 +120,7 @@ class SyntheticLlama:
 
     @torch.no_grad()
     def forward(self, batch) -> torch.Tensor:
-        """Hidden states of every token -> logits of each sequence's LAST token, [B, vocab]."""
+        """Hidden states of every token -> logits of each sequence's LAST token, [B, vocab]; of every node for draft trees, [T, vocab]."""
         x = F.embedding(batch.input_ids, self.embed)
         residual = None
         pos, loc = batch.positions, batch.out_cache_loc

@@ -2,17 +2,27 @@
 dispatch to `batch.attn_backend.forward(q=, k=, v=, layer=, batch=)`."""
 from __future__ import annotations
 
+from typing import Optional
+
+import torch
 import torch.nn as nn
 
 
 class Attention(nn.Module):
-    def __init__(self, layer_id: int, num_heads: int, num_kv_heads: int, head_dim: int, scale: float = 1.0):
+    def __init__(self, layer_id: int, num_heads: int, num_kv_heads: int, head_dim: int, scale: float = 1.0, *,
+                 logit_cap: float = 0.0, window: int = 0, slopes: Optional[torch.Tensor] = None):
+        """logit_cap > 0 caps the scores (s -> logit_cap * tanh(s / logit_cap)), window > 0 lets a token see that many keys, its
+        own included, and slopes (fp32 [num_heads], on the device) biases them by -slope * distance.  The reference's layers
+        have none of the three."""
         super().__init__()
         self.layer_id = layer_id
         self.num_heads = num_heads
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
         self.scale = scale          # kept for interface parity; the reference never forwards it to SDPA
+        self.logit_cap = float(logit_cap)
+        self.window = int(window)
+        self.slopes = slopes
 
     def forward(self, q, k, v, batch):
         return batch.attn_backend.forward(q=q, k=k, v=v, layer=self, batch=batch)

@@ -10,6 +10,10 @@ flash_attention_backend.py:44-151):
 
 It works with this package's Batch (host mirrors of the lengths ride along, so no device sync happens) and
 with the reference's own Batch (then lengths are read back once per forward, as its FA3 backend does).
+
+Beyond the reference: layers with a score cap, a distance bias or a window (Attention.logit_cap / slopes / window), batches with
+a document or prefix mask (batch.doc_starts / bidir_lens) and batches that verify draft trees (Batch.prepare_for_tree) go to the
+scored-attention kernels (ops.scored_attn, ops.tree_attn); everything else takes the paths it always took.
 """
 from __future__ import annotations
 
@@ -32,6 +36,7 @@ class ForwardMetadata:
     workspace: Optional[torch.Tensor] = None
     ws: Optional[torch.Tensor] = None              # planned decode: the workspace of this forward ...
     ws_key: Optional[tuple] = None                 # ... and the (B, Hq, Hkv, D) it was sized for
+    tree: bool = False                             # a batch of draft trees
     first_layer: Optional[int] = None              # layer_id of the first layer that used this metadata
 
 
@@ -60,6 +65,19 @@ def _pad_groups(q: torch.Tensor, Hkv: int, G: int, Gp: int, D: int) -> torch.Ten
 def _drop_pad(o: torch.Tensor, Hkv: int, G: int, Gp: int, D: int) -> torch.Tensor:
     T = o.shape[0]
     return o.view(T, Hkv, Gp, D)[:, :, :G].reshape(T, Hkv * G * D)
+
+
+def _modifiers(layer) -> dict:
+    """The score modifiers of a layer as ops.scored_attn takes them; a reference layer has none."""
+    return {"softcap": getattr(layer, "logit_cap", 0.0), "slopes": getattr(layer, "slopes", None), "window": getattr(layer, "window", 0)}
+
+
+def _masks(batch) -> dict:
+    return {"doc_starts": getattr(batch, "doc_starts", None), "bidir_lens": getattr(batch, "bidir_lens", None)}
+
+
+def _any(options: dict) -> bool:
+    return any(v is not None and (isinstance(v, torch.Tensor) or bool(v)) for v in options.values())
 
 
 class MI355AttnBackend:
@@ -97,6 +115,9 @@ class MI355AttnBackend:
         lens = getattr(batch, "seq_lens_host", None)
         if lens is None:
             lens = [int(x) for x in batch.seq_lens.tolist()]          # one sync, like flash_attention_backend.py:60
+        if getattr(batch, "tree", None) is not None:
+            self.forward_metadata = ForwardMetadata(decode=False, max_seq_len=max(batch.tree_lens_host), tree=True)
+            return
         if batch.mode.is_decode():
             self.forward_metadata = ForwardMetadata(decode=True, max_seq_len=max(lens))
             self._plan_key = (batch, sum(lens))       # the plan itself needs the layer's head shape: built lazily
@@ -122,6 +143,8 @@ class MI355AttnBackend:
 
     # ---- per layer ------------------------------------------------------------------------------
     def forward(self, q, k, v, layer, batch):
+        if getattr(batch, "tree", None) is not None:
+            return self.forward_tree(q, k, v, layer, batch)
         if batch.mode.is_decode():
             return self.forward_decode(q, k, v, layer, batch)
         return self.forward_extend(q, k, v, layer, batch)
@@ -150,6 +173,9 @@ class MI355AttnBackend:
             md.first_layer = layer.layer_id
         k_pool, v_pool = batch.kvcache.get_kv_cache(layer.layer_id)
         B = q.shape[0]
+        mods, masks = _modifiers(layer), _masks(batch)
+        if _any(mods) or _any(masks):
+            return self._scored(q, k, v, layer, batch, mods, masks, {})
         fuse = (self.fused_store and k is not None and k.dtype == k_pool.dtype
                 and v.dtype == v_pool.dtype and k.stride(-1) == 1 and v.stride(-1) == 1)
         if not fuse:
@@ -175,12 +201,44 @@ class MI355AttnBackend:
                                     k_new=k if fuse else None, v_new=v if fuse else None)
         return o if Gp == G else _drop_pad(o, Hkv, G, Gp, D)
 
+    def _scored(self, q, k, v, layer, batch, mods, masks, form):
+        """Decode or extend attention with modified scores; `form` holds the ragged form's arguments."""
+        self._store_kv(k, v, layer, batch)
+        k_pool, v_pool = batch.kvcache.get_kv_cache(layer.layer_id)
+        md = self.forward_metadata
+        need = ops.scored_workspace_bytes(batch.seq_lens.numel(), q.shape[0], layer.num_heads, layer.num_kv_heads, layer.head_dim,
+                                          form.get("max_extend_len", 1), md.max_seq_len, mods["window"])
+        return ops.scored_attn(q, k_pool, v_pool, batch.page_manager.page_table, batch.page_table_ids, batch.seq_lens, self.page_size,
+                               layer.num_heads, md.max_seq_len, workspace=self._ws(need, q.device), **form, **mods, **masks)
+
+    def forward_tree(self, q, k, v, layer, batch):
+        """Attention of a batch of draft trees (Batch.prepare_for_tree): every node over its request's cached tokens and its
+        ancestors, after the nodes' K/V have been written to their slots."""
+        md = self.forward_metadata
+        if md is None or not md.tree or self._new_forward(md, layer):
+            self.init_forward_metadata(batch)
+            md = self.forward_metadata
+            md.first_layer = layer.layer_id
+        mods = _modifiers(layer)
+        if mods.pop("window"):
+            raise ops._lib.MI355AttnError("MI355AttnBackend: draft trees are not supported in layers with a window")
+        self._store_kv(k, v, layer, batch)
+        k_pool, v_pool = batch.kvcache.get_kv_cache(layer.layer_id)
+        need = ops.scored_workspace_bytes(batch.seq_lens.numel(), q.shape[0], layer.num_heads, layer.num_kv_heads, layer.head_dim,
+                                          batch.tree.max_nodes, md.max_seq_len)
+        return ops.tree_attn(q, k_pool, v_pool, batch.page_manager.page_table, batch.page_table_ids, batch.seq_lens, batch.tree, self.page_size,
+                             layer.num_heads, md.max_seq_len, workspace=self._ws(need, q.device), **mods)
+
     def forward_extend(self, q, k, v, layer, batch):
         md = self.forward_metadata
         if md is None or md.decode or self._new_forward(md, layer):
             self.init_forward_metadata(batch)
             md = self.forward_metadata
             md.first_layer = layer.layer_id
+        mods, masks = _modifiers(layer), _masks(batch)
+        if _any(mods) or _any(masks):
+            return self._scored(q, k, v, layer, batch, mods, masks,
+                                {"prefix_lens": batch.prefix_lens, "cu_q": md.cu_q, "max_extend_len": md.max_extend_len})
         self._store_kv(k, v, layer, batch)       # first: the new tokens' K/V are read back from the pool
         k_pool, v_pool = batch.kvcache.get_kv_cache(layer.layer_id)
         T = q.shape[0]

@@ -27,12 +27,16 @@ from . import ops
 class Mode(Enum):
     PREFILL = "prefill"
     DECODE = "decode"
+    TREE = "tree"                          # a verification step over drafted tokens (no counterpart in the reference)
 
     def is_decode(self):
         return self == Mode.DECODE
 
     def is_prefill(self):
         return self == Mode.PREFILL
+
+    def is_tree(self):
+        return self == Mode.TREE
 
 
 @dataclasses.dataclass
@@ -207,6 +211,14 @@ class Batch:
         self.prefix_lens_host: Optional[List[int]] = None
         self.cu_q: Optional[torch.Tensor] = None            # int32 [B+1], prefill only
         self.row_of_token: Optional[torch.Tensor] = None    # int64 [T], prefill only
+        # masks of ONE forward (ops.scored_attn), to be set between prepare_for_* and the forward: every prepare clears them
+        self.doc_starts: Optional[torch.Tensor] = None      # int32 [T]: first position of every token's document
+        self.bidir_lens: Optional[torch.Tensor] = None      # int32 [B]: a prompt prefix that attends both ways
+        # draft trees (prepare_for_tree .. commit_tree)
+        self.tree: Optional[ops.TreePlan] = None
+        self.tree_lens_host: Optional[List[int]] = None     # cached tokens + nodes
+        self._tree_parents: List[List[int]] = []
+        self._tree_pages: List[List[int]] = []
 
     def is_empty(self):
         return len(self.reqs) == 0
@@ -214,9 +226,13 @@ class Batch:
     def batch_size(self):
         return len(self.reqs)
 
+    def _begin(self, mode: Mode) -> None:
+        self._no_open_tree()
+        self.mode, self.doc_starts, self.bidir_lens = mode, None, None
+
     # ---- prefill (engine/batch.py:244-317)
     def prepare_for_prefill(self) -> None:
-        self.mode = Mode.PREFILL
+        self._begin(Mode.PREFILL)
         plan = plan_prefill(self.reqs, self.page_manager, self.kvcache)
         B, T = len(self.reqs), plan.T
         i64 = _h2d(np.concatenate([plan.input_ids, np.asarray(plan.rows, dtype=np.int64),
@@ -233,7 +249,7 @@ class Batch:
 
     # ---- decode (engine/batch.py:319-343)
     def prepare_for_decode(self) -> None:
-        self.mode = Mode.DECODE
+        self._begin(Mode.DECODE)
         if self.seq_lens_host is None:
             self.seq_lens_host = [int(x) for x in self.seq_lens.tolist()]
         self.input_ids = self.output_ids
@@ -261,8 +277,78 @@ class Batch:
             raise RuntimeError("KV pool exhausted during decode (call check_decode_mem / retract_decode first)")
         self.seq_lens_host = (lens + 1).tolist()
 
+    # ---- draft trees (speculative decoding; no counterpart in the reference)
+    def prepare_for_tree(self, draft_ids: List[List[int]], parents: List[List[int]]) -> None:
+        """A verification step: request b brings the tokens draft_ids[b] as a tree, parents[b][j] being the index of token j's
+        parent, below j, or -1 for a token that follows the cached ones directly (usually one: the token sampled last).  Nodes take the
+        request's next slots in their order and the position of their depth.  One allocation, two copies, one launch.  The forward
+        then gives a row of logits per node; commit_tree keeps a path."""
+        if len(draft_ids) != len(self.reqs) or len(parents) != len(self.reqs):
+            raise ValueError("prepare_for_tree: one tree per request")
+        for ids, par in zip(draft_ids, parents):
+            if len(ids) != len(par) or not ids or any(not -1 <= p < j for j, p in enumerate(par)):
+                raise ValueError("prepare_for_tree: a tree needs a token and a parent below it (or -1) per node, and at least one node")
+        nodes = [len(ids) for ids in draft_ids]
+        if max(nodes) > ops.TREE_MAX_NODES:
+            raise ValueError(f"prepare_for_tree: trees of up to {ops.TREE_MAX_NODES} nodes are supported")
+        ps, held = self.page_size, list(self._lens_host())
+        lens = [p + n for p, n in zip(held, nodes)]
+        width = getattr(self.page_manager, "max_page_num", None)
+        if width is not None and -(-max(lens) // ps) > width:
+            raise RuntimeError(f"a tree would reach token {max(lens)}: more than the page table's {width} columns (max_context_len)")
+        if sum(-(-n // ps) - -(-p // ps) for n, p in zip(lens, held)) > self.kvcache.available_page_num():
+            raise RuntimeError("KV pool exhausted by draft trees (call check_decode_mem / retract_decode first)")
+        self._begin(Mode.TREE)
+        self._tree_pages = self.kvcache.allocate_pages_prefill(lens, held)
+        self._tree_parents = [list(p) for p in parents]
+        self.tree_lens_host = lens
+        cu, off = np.concatenate([[0], np.cumsum(nodes)]), np.concatenate([[0], np.cumsum([len(p) for p in self._tree_pages])])
+        B, T, n_new = len(nodes), int(cu[-1]), int(off[-1])
+        i32 = _h2d(np.concatenate([np.concatenate(self._tree_parents), cu, off, np.concatenate([np.asarray(p, dtype=np.int64) for p in self._tree_pages])])
+                   .astype(np.int32), self.device)
+        self.input_ids = _h2d(np.concatenate([np.asarray(i, dtype=np.int64) for i in draft_ids]), self.device)
+        self.output_ids = None
+        self.tree = ops.tree_prepare(self.page_manager.page_table, self.page_table_ids, self.seq_lens, i32[:T], i32[T:T + B + 1], ps, max(nodes),
+                                     new_pages=i32[T + 2 * (B + 1):T + 2 * (B + 1) + n_new], new_page_off=i32[T + B + 1:T + 2 * (B + 1)])
+        self.positions, self.out_cache_loc, self.cu_q, self.row_of_token = self.tree.positions, self.tree.out_cache_loc, self.tree.cu_q, None
+
+    def commit_tree(self, accepted: List[List[int]]) -> None:
+        """Ends a verification step: request b keeps the nodes accepted[b], a path from a root downwards (may be empty).  Their
+        K/V move to the slots of their positions, the other nodes' pages go back to the pool, the lengths grow by the paths."""
+        if self.tree is None:
+            raise RuntimeError("commit_tree: no tree is open")
+        for path, par in zip(accepted, self._tree_parents):
+            if any(not 0 <= n < len(par) for n in path) or any(par[n] != (path[i - 1] if i else -1) for i, n in enumerate(path)):
+                raise ValueError("commit_tree: a path starts at a root and goes from parent to child")
+        if len(accepted) != len(self.reqs):
+            raise ValueError("commit_tree: one path per request")
+        ps, held, first = self.page_size, self._lens_host(), 0
+        src, dst, lens, back = [], [], [], []
+        for path, par, p, pages in zip(accepted, self._tree_parents, held, self._tree_pages):
+            for depth, n in enumerate(path):
+                if n != depth:
+                    src.append(first + n), dst.append(first + depth)
+            lens.append(p + len(path))
+            back.extend(pages[max(0, -(-lens[-1] // ps) - -(-p // ps)):])
+            first += len(par)
+        if src:
+            at = _h2d(np.asarray([dst, src], dtype=np.int64), self.device)
+            slots = self.out_cache_loc[at]
+            self.kvcache.move_tokens(slots[0], slots[1])
+        if back:
+            self.kvcache._free_pages(back)
+        self.seq_lens_host = lens
+        self.seq_lens = _h2d(np.asarray(lens, dtype=np.int64), self.device)
+        self.tree = self.tree_lens_host = self.cu_q = self.positions = self.out_cache_loc = self.input_ids = None
+        self._tree_parents, self._tree_pages, self.mode = [], [], Mode.DECODE
+
     # ---- bookkeeping kept working (engine/batch.py:345-464)
+    def _no_open_tree(self) -> None:
+        if self.tree is not None:
+            raise RuntimeError("a draft tree is open: commit_tree first")
+
     def filter_batch(self, keep_indices: Optional[List[int]] = None) -> None:
+        self._no_open_tree()
         if keep_indices is None:
             keep_indices = [i for i, r in enumerate(self.reqs) if not r.finished()]
         if not keep_indices:
@@ -286,6 +372,7 @@ class Batch:
             self.prefix_lens_host = [self.prefix_lens_host[i] for i in keep_indices]
 
     def merge_batch(self, other: "Batch") -> None:
+        self._no_open_tree(), other._no_open_tree()
         self.page_table_ids = torch.cat([self.page_table_ids, other.page_table_ids])
         self.seq_lens = torch.cat([self.seq_lens, other.seq_lens])
         if self.prefix_lens is not None and other.prefix_lens is not None:
@@ -320,6 +407,7 @@ class Batch:
         """Give the pages of the most recently started requests back until the rest can keep decoding
         (batch.py:393-464, with its undefined `residual_size` resolved to the evident max(0, .) clamp, and the request's
         partly filled last page returned too: the reference's floor at :428-431 leaks it)."""
+        self._no_open_tree()
         order = sorted(range(len(self.reqs)),
                        key=lambda i: (len(self.reqs[i].output_ids), -len(self.reqs[i].origin_input_ids)), reverse=True)
         lens = self._lens_host()

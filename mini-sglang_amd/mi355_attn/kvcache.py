@@ -115,5 +115,11 @@ class KVCache:
         """k_cache[layer][loc] = cache_k; v_cache[layer][loc] = cache_v (kvcache.py:69-79), one HIP launch."""
         ops.kv_store(self.k_cache[layer_id], self.v_cache[layer_id], loc, cache_k, cache_v)
 
+    def move_tokens(self, dst: torch.Tensor, src: torch.Tensor) -> None:
+        """K and V of slots `src` to slots `dst` (int64), in every layer; the two may overlap, all of `src` is read first."""
+        for layer in range(self.layer_num):
+            k, v = self.k_cache[layer], self.v_cache[layer]
+            self.write_kv(layer, dst, k[src], v[src])
+
     def get_kv_cache(self, layer_id: int) -> Tuple[torch.Tensor, torch.Tensor]:
         return self.k_cache[layer_id], self.v_cache[layer_id]

@@ -527,6 +527,9 @@ def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, pag
     return out
 
 
+TREE_MAX_NODES = _lib.TREE_MAX_NODES
+
+
 class TreePlan(NamedTuple):
     """What tree_prepare makes once per verification step, for every layer's tree_attn."""
     mask: torch.Tensor                 # int32 [T, words]: bit x of word w = node 32 w + x is the row's node or an ancestor
