@@ -261,11 +261,11 @@ int m355_rope_kv_store(void *q, int64_t q_row_stride, void *k, int64_t k_row_str
  * length 0 gives zeros).  Any Hq that is a multiple of Hkv; head_dim 64 or 128; bf16 or fp16.
  * S = token rows of the pools (< 2^31); pt_rows / pt_cols = the table's shape.  Whatever the tables hold, nothing outside the
  * pools, the table and the T rows is read: ids and pages out of range are brought back into it.
- * max_extend_len >= the longest cu_q[b+1] - cu_q[b] (rows past it are not computed); max_seq_len_hint and window size the
- * launch.  workspace: m355_scored_workspace_bytes bytes (the same B ... window), 256-byte aligned, may be NULL where that is 0;
- * calls that overlap need one each. */
+ * max_extend_len >= the longest cu_q[b+1] - cu_q[b] (rows past it are not computed); max_seq_len_hint >= the longest
+ * request, for the choice of the launch.  workspace: m355_scored_workspace_bytes bytes (the same sizes), 256-byte aligned, may be
+ * NULL where that is 0; calls that overlap need one each. */
 int64_t m355_scored_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_extend_len,
-                                    int32_t max_seq_len_hint, int32_t window);
+                                    int32_t max_seq_len_hint);
 int m355_scored_attn(const void *q, int64_t q_row_stride, const void *k_pool, const void *v_pool, int64_t pool_row_stride,
                      int64_t S, const int32_t *page_table, int64_t pt_row_stride, int32_t pt_rows, int32_t pt_cols,
                      const int64_t *page_table_ids, const int64_t *seq_lens, const int64_t *prefix_lens, const int32_t *cu_q,
@@ -290,8 +290,7 @@ int m355_tree_prepare(int32_t *page_table, int64_t pt_row_stride, int32_t pt_row
                       uint32_t *tree_mask, int32_t mask_words, int64_t *positions, int64_t *out_cache_loc, void *stream);
 
 /* Attention of the trees' nodes: node t sees the request's prefix_lens[b] cached tokens and the nodes of its mask row (their
- * K/V already in the pools).  Scores, zeros, bounds, workspace (m355_scored_workspace_bytes with max_extend_len = max_nodes,
- * window = 0) as m355_scored_attn; max_seq_len_hint >= the longest prefix + nodes; positions is read for the bias only
+ * K/V already in the pools).  Scores, zeros, bounds, workspace (m355_scored_workspace_bytes with max_extend_len = max_nodes) as m355_scored_attn; max_seq_len_hint >= the longest prefix + nodes; positions is read for the bias only
  * (distance = difference of depths) and may be NULL without slopes. */
 int m355_tree_attn(const void *q, int64_t q_row_stride, const void *k_pool, const void *v_pool, int64_t pool_row_stride, int64_t S,
                    const int32_t *page_table, int64_t pt_row_stride, int32_t pt_rows, int32_t pt_cols,

@@ -24,6 +24,16 @@
 
 namespace m355 {
 
+// (request, kv head) unit u as one share, without splits
+__device__ __forceinline__ Share whole_request(const ScoredParams& p, int u) {
+    Share s = {};
+    s.any = true;
+    s.b = u / p.Hkv; s.h = u % p.Hkv; s.nsp = 1; s.chunk = 0x3fffffc0;
+    s.r = load_span(p, s.b);
+    s.pt_row = table_row(p, s.b);
+    return s;
+}
+
 // the range of the rows of 16 neighbouring lanes, in all of them
 template <int CTRL>
 __device__ __forceinline__ BlockRange join_dpp(BlockRange a) {
@@ -48,7 +58,7 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 // (16 requests of 20 000 to 32 768 tokens, 222 MB: 41.6 us, 5.3 TB/s; with four waves 49.8, with one 58.7).  More rows go to
 // the other kernel: with 32 rows here, 16 requests of 2 250 tokens took 45 us against 29.
 // ------------------------------------------------------------------------------------------------------------------------
-constexpr int kFewRows = 16, kFewWaves = 2;
+constexpr int kFewRows = 16, kFewWaves = 2, kWideRows = 128;
 constexpr int kFewSlots = 1024;                       // tokens whose pool slots are in LDS at a time
 
 template <int D, bool MOD, bool F16>
@@ -62,13 +72,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
     const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
 
-    // ---- which rows and keys.  The kv head rotates with the unit: workgroups go round the 8 XCDs, and an XCD should not read one
-    // head's column of the pools only.
-    const int u = blockIdx.x, h = (u + u / p.Hkv) % p.Hkv, b = u / p.Hkv % p.B, sp = u / (p.Hkv * p.B);
-    const ReqSpan r = load_span(p, b);
+    const Share sh = p.slots ? find_share<kFewRows, true>(p) : whole_request(p, blockIdx.x);
+    if (!sh.any) return;
+    const int h = sh.h, b = sh.b, sp = sh.sp;
+    const ReqSpan r = sh.r;
     const int rows = r.E * p.G;
     if (rows == 0) return;
-    const int32_t* pt_row = table_row(p, b);
+    const int32_t* pt_row = sh.pt_row;
     const bool ok = n < rows;
     const int j = ok ? n / p.G : 0, g = ok ? n - j * p.G : 0;
     const int64_t t = r.q0 + j;
@@ -89,9 +99,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
     const int lo_min = __builtin_amdgcn_readfirstlane(br.lo_min), hi_max = __builtin_amdgcn_readfirstlane(br.hi_max);
     const int lo_max = __builtin_amdgcn_readfirstlane(br.lo_max), hi_min = __builtin_amdgcn_readfirstlane(br.hi_min);
     const int first = lo_min & ~31, keys = lo_min < hi_max ? hi_max - first : 0;
-    const int active = imax(1, imin(p.splits, (keys + p.chunk - 1) / p.chunk));
+    const int active = imax(1, imin(sh.nsp, (keys + sh.chunk - 1) / sh.chunk));
     if (sp >= active) return;
-    const int t0 = first + sp * p.chunk, t1 = keys ? (sp == active - 1 ? hi_max : t0 + p.chunk) : t0;
+    const int t0 = first + sp * sh.chunk, t1 = keys ? (sp == active - 1 ? hi_max : t0 + sh.chunk) : t0;
     const float slope = MOD && p.slopes ? p.slopes[h * p.G + g] * kLog2e : 0.f;
 
     bf16x8 qf[M::KS];
@@ -274,7 +284,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
         const int row = m / p.G, head = h * p.G + m - row * p.G;
         const int64_t item = (int64_t)(r.q0 + row) * p.Hq + head;
         if (active > 1) {
-            float* wo = p.part + (item * p.splits + sp) * (D + 4);
+            float* wo = p.part + ((int64_t)(sh.part0 + sp) * kFewRows + m) * (D + 4);
             *reinterpret_cast<f32x4*>(wo + 4 * ch) = o;
             if (ch == 0) *reinterpret_cast<float2*>(wo + D) = make_float2(mx, l);
         } else {
@@ -283,7 +293,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
             if (l != 0.f) w = make_uint2(pack16<F16>(o[0] * inv, o[1] * inv), pack16<F16>(o[2] * inv, o[3] * inv));
             *reinterpret_cast<uint2*>(p.out + (int64_t)(r.q0 + row) * p.o_stride + (int64_t)head * D + 4 * ch) = w;
         }
-        if (sp == 0 && ch == 0 && p.splits > 1) p.part_n[item] = active;
+        if (sp == 0 && ch == 0 && p.slots) p.part_of[item] = make_int2(sh.part0 * kFewRows + m, active);
     }
 }
 
@@ -299,29 +309,37 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     constexpr int NW = 4, NBUF = 4;
     constexpr int NT = 64 * NW, ROWS = 32 * NW, IPW = 2 * W::NI / NW, HP = IPW / 2;
     constexpr int NP = NBUF / 2;                      // pairs the ring holds: NP - 1 are on their way while one is worked on
-    static_assert(IPW % 2 == 0 && W::NI % NW == 0 && NP == 2 && NBUF * W::TILEB <= 65536, "ring geometry");
+    static_assert(IPW % 2 == 0 && W::NI % NW == 0 && NP == 2 && NBUF * W::TILEB <= 65536 && ROWS == kWideRows, "ring geometry");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[NBUF * W::BUFB];      // NBUF K tiles, NBUF V tiles
     __shared__ int32_t slotw[kSlotWin];
     __shared__ int32_t wlim[NW][2];
     const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int l = threadIdx.x & 63, c = l & 31, hh = l >> 5;
 
-    // ---- which rows: all row blocks of one (request, kv head), which walk much the same keys, on one XCD, the last (longest
-    // under a causal mask) first; pairs left over after the full rounds of 8 are spread over all XCDs
-    const int n_bh = p.B * p.Hkv, mapped = (n_bh >> 3) * 8 * p.blocks;
-    int tb, bh;
-    if ((int)blockIdx.x < mapped) {
-        const int item = blockIdx.x >> 3;
-        tb = p.blocks - 1 - item % p.blocks; bh = (item / p.blocks) * 8 + (blockIdx.x & 7);
+    // ---- which rows and keys.  Without splits: all row blocks of one (request, kv head), which walk much the same keys, on one XCD,
+    // the last (longest under a causal mask) first; pairs left over after the full rounds of 8 are spread over all XCDs
+    Share sh;
+    if (p.slots) {
+        sh = find_share<ROWS, false>(p);
+        if (!sh.any) return;
     } else {
-        const int item = blockIdx.x - mapped;
-        tb = p.blocks - 1 - item % p.blocks; bh = (n_bh & ~7) + item / p.blocks;
+        const int n_bh = p.B * p.Hkv, mapped = (n_bh >> 3) * 8 * p.blocks;
+        int tb, bh;
+        if ((int)blockIdx.x < mapped) {
+            const int item = blockIdx.x >> 3;
+            tb = p.blocks - 1 - item % p.blocks; bh = (item / p.blocks) * 8 + (blockIdx.x & 7);
+        } else {
+            const int item = blockIdx.x - mapped;
+            tb = p.blocks - 1 - item % p.blocks; bh = (n_bh & ~7) + item / p.blocks;
+        }
+        sh = whole_request(p, bh);
+        sh.rb = tb;
     }
-    const int h = bh % p.Hkv, b = bh / p.Hkv, sp = blockIdx.y;
-    const ReqSpan r = load_span(p, b);
+    const int h = sh.h, b = sh.b, sp = sh.sp, tb = sh.rb;
+    const ReqSpan r = sh.r;
+    const int32_t* pt_row = sh.pt_row;
     const int rows = r.E * p.G;
     if (ROWS * tb >= rows) return;                                 // whole workgroup: no barrier has been reached yet
-    const int32_t* pt_row = table_row(p, b);
 
     // ---- this lane's row and the limits of its wave and workgroup
     const int row0 = ROWS * tb + 32 * wid, mrow = row0 + c;
@@ -381,8 +399,8 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     lo_wg = __builtin_amdgcn_readfirstlane(lo_wg); hi_wg = __builtin_amdgcn_readfirstlane(hi_wg);
     const bool none = lo_wg >= hi_wg;
     const int pair0 = none ? 0 : lo_wg >> 6, pairs_end = none ? 0 : (hi_wg + 63) >> 6, n_tiles = (hi_wg + 31) >> 5;
-    const int per = p.chunk >> 6;
-    const int active = imax(1, imin(p.splits, (pairs_end - pair0 + per - 1) / per));
+    const int per = sh.chunk >> 6;
+    const int active = imax(1, imin(sh.nsp, (pairs_end - pair0 + per - 1) / per));
     if (sp >= active) return;
     const int p_begin = pair0 + sp * per, n_pairs = sp == active - 1 ? pairs_end : p_begin + per;   // exclusive end
 
@@ -625,9 +643,10 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     const float lt = la + lb;
     const int64_t item = t * p.Hq + h * p.G + g;
     if (!valid) return;
-    if (p.splits > 1 && sp == 0 && hh == 0) p.part_n[item] = active;
+    const int prow = 32 * wid + c;                                 // row inside the block
+    if (p.slots && sp == 0 && hh == 0) p.part_of[item] = make_int2(sh.part0 * ROWS + prow, active);
     if (active > 1) {                                              // unnormalised partial of this split: O^T, m, l
-        float* wo = p.part + (item * p.splits + sp) * (D + 4);
+        float* wo = p.part + ((int64_t)(sh.part0 + sp) * ROWS + prow) * (D + 4);
 #pragma unroll
         for (int dt = 0; dt < W::DT; ++dt)
 #pragma unroll
@@ -650,9 +669,9 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
         }
 }
 
-// out[row, head, :] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the splits that hold a part: D/4 lanes per (row, head),
-// four floats each, eight splits' loads in flight per lane.
-template <int D, bool F16>
+// out[row, head, :] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the parts of a row, RB part rows apart: D/4 lanes per
+// (row, head), four floats each, eight parts' loads in flight per lane.
+template <int D, int RB, bool F16>
 __global__ __launch_bounds__(256) void scored_merge_kernel(const ScoredParams p) {
     constexpr int LPI = D / 4, CH = 8;
     const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPI;
@@ -660,25 +679,22 @@ __global__ __launch_bounds__(256) void scored_merge_kernel(const ScoredParams p)
     const int64_t row = item / p.Hq, head = item - row * p.Hq;
     const int64_t r0 = p.cu_q ? imax(p.cu_q[0], 0) : 0, r1 = p.cu_q ? imin(p.cu_q[p.B], p.T) : imin(p.B, p.T);
     if (row < r0 || row >= r1) return;                              // rows of no request: left as they were
-    // The first eight parts are requested together with their number: parts that nobody wrote are left out by selection, never
-    // by a factor.
-    const float* base = p.part + item * p.splits * (D + 4);
-    const int held = p.part_n[item];
+    const int2 of = p.part_of[item];
+    const int n = of.y;
+    // 1: written by the attention kernel.  (A row that no share reached - lengths that contradict cu_q - has no entry: nothing out of
+    // the parts is read for it.)
+    if (n <= 1 || of.x < 0 || of.x / RB + (int64_t)n > p.max_parts) return;
+    const float* base = p.part + (int64_t)of.x * (D + 4);
     float mx = -INFINITY, den = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    int n = p.splits;
     for (int s0 = 0; s0 < n; s0 += CH) {
         float2 ml[CH];
         f32x4 o[CH];
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
-            const float* ps = base + (int64_t)imin(s0 + k, n - 1) * (D + 4);
+            const float* ps = base + (int64_t)imin(s0 + k, n - 1) * (RB * (D + 4));
             ml[k] = *reinterpret_cast<const float2*>(ps + D);
             o[k] = *reinterpret_cast<const f32x4*>(ps + 4 * li);
-        }
-        if (s0 == 0) {
-            n = imin(held, p.splits);
-            if (n <= 1) return;                                     // written by the attention kernel
         }
         float mn = mx;
 #pragma unroll
@@ -713,42 +729,35 @@ static int shift_of(int32_t x) {
     return s;
 }
 
-// How a call is cut, from its sizes alone (so that the workspace query and the launch agree).
-//
-// The rows a request brings choose the kernel.  Keys are split where there are fewer (request, kv head, row block) units than
-// workgroups the chip holds at once: two a CU (four of the small ones at head_dim 64).  One round of equal splits is what
-// pays: more, shorter ones cost a start of ~5 us each and parts to join (16 trees of 32 nodes over 2 250 tokens: 4 splits 38.2 +
-// 8.7 us, 8 splits 50.8 + 12.7, none 58.1).  A split is at least 256 keys, or a sixteenth of the range where that is shorter - a
-// single short request is a matter of latency (8 nodes over 700 tokens: 64 keys 9.8 + 4.2 us, 128 keys 13.4 + 3.5, 256 keys
-// 15.6 + 3.8; over 4 250 tokens: 256 keys 12.3 + 4.8, 128 keys 11.8 + 6.3).
-struct ScoredCut { bool wide; int32_t blocks, splits, chunk; int64_t part_bytes, bytes; };
-static ScoredCut scored_cut(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int32_t D, int64_t ext, int64_t max_len, int64_t window) {
+// How a call is cut, from its sizes alone (so that the workspace query and the launch agree).  The rows a request brings choose the
+// kernel.  Keys are split where there are fewer (request, kv head, row block) units than twice the workgroups that the chip
+// holds at once; find_share then lays out the parts.  A part is at least 256 keys (128 in the few-row kernel), or a sixteenth of the
+// request where that is shorter: a single short request is a matter of latency (8 nodes over 700 tokens: 64 keys 9.8 + 4.2 us,
+// 128 keys 13.4 + 3.5, 256 keys 15.6 + 3.8; over 4 250 tokens: 256 keys 12.3 + 4.8, 128 keys 11.8 + 6.3).
+struct ScoredCut { bool wide; int32_t blocks, slots, max_parts; int64_t grid, part_bytes, bytes; };
+static ScoredCut scored_cut(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int32_t D, int64_t ext, int64_t max_len) {
+    constexpr int64_t kCus = 256;
     ScoredCut c = {};
     const int64_t G = Hq / Hkv;
     if (ext > T) ext = T;
-    const int64_t rows = ext * G, per_block = rows > kFewRows ? 128 : kFewRows;
+    const int64_t rows = ext * G, rb = rows > kFewRows ? kWideRows : kFewRows;
     c.wide = rows > kFewRows;
-    c.blocks = (int32_t)((rows + per_block - 1) / per_block);
-    int64_t span = window > 0 && window + ext < max_len ? window + ext : max_len;
-    span += 63;                                                     // the first tile may begin before the first visible key
+    c.blocks = (int32_t)((rows + rb - 1) / rb);
+    // workgroups a CU holds: two by the LDS at head_dim 128, three by the registers and four by the LDS at 64
+    const int64_t slots = kCus * (D == 128 ? 2 : (c.wide ? 3 : 4));
     // (a ragged batch has fewer row blocks than its longest request suggests)
-    int64_t units = B * Hkv * c.blocks;
-    const int64_t packed = Hkv * ((T * G + per_block - 1) / per_block + B);
-    if (packed < units) units = packed;
-    int64_t splits = (c.wide || D == 128 ? 512 : 1024) / units;
-    if (splits < 1) splits = 1;
-    int64_t shortest = span / 16;
-    if (shortest > 256) shortest = 256;
-    int64_t chunk = (span + splits - 1) / splits;
-    if (chunk < shortest) chunk = shortest;
-    chunk = (chunk + 63) / 64 * 64;
-    splits = (span + chunk - 1) / chunk;
-    c.splits = (int32_t)splits;
-    c.chunk = (int32_t)chunk;
-    if (splits > 1) {
-        c.part_bytes = T * Hq * splits * (D + 4) * (int64_t)sizeof(float);
-        c.bytes = c.part_bytes + T * Hq * (int64_t)sizeof(int32_t);
-    }
+    int64_t blocks = B * c.blocks;
+    const int64_t packed = (T * G + rb - 1) / rb + B;
+    if (packed < blocks) blocks = packed;
+    c.grid = B * Hkv * c.blocks;
+    if (blocks * Hkv >= 2 * slots || max_len <= 64) return c;
+    c.slots = (int32_t)slots;
+    const int64_t units = blocks * Hkv, full = (int64_t)full_parts((float)slots, (float)units, !c.wide);
+    const int64_t low = Hkv & -Hkv, rounding = c.blocks > 1 ? 8 / (low < 8 ? low : 8) / 2 * units : 0;
+    c.max_parts = (int32_t)(full + units + rounding + 16);
+    c.grid = c.max_parts;
+    c.part_bytes = c.max_parts * rb * (D + 4) * (int64_t)sizeof(float);
+    c.bytes = c.part_bytes + T * Hq * (int64_t)sizeof(int2);
     return c;
 }
 
@@ -770,27 +779,28 @@ static int check_common(const ScoredParams& p, int32_t max_extend_len, int32_t m
 template <int D, bool MOD, bool F16>
 static void launch_kernels(const ScoredParams& p, const ScoredCut& c, hipStream_t st) {
     if (c.wide) {
-        hipLaunchKernelGGL((scored_wide_kernel<D, MOD, F16>), dim3((unsigned)(p.B * p.Hkv * p.blocks), (unsigned)p.splits), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((scored_wide_kernel<D, MOD, F16>), dim3((unsigned)c.grid), dim3(256), 0, st, p);
     } else {
-        hipLaunchKernelGGL((scored_few_kernel<D, MOD, F16>), dim3((unsigned)((int64_t)p.splits * p.B * p.Hkv)), dim3(64 * kFewWaves), 0, st, p);
+        hipLaunchKernelGGL((scored_few_kernel<D, MOD, F16>), dim3((unsigned)c.grid), dim3(64 * kFewWaves), 0, st, p);
     }
-    if (p.splits > 1) {
-        const int64_t lanes = (int64_t)p.T * p.Hq * (D / 4);
-        hipLaunchKernelGGL((scored_merge_kernel<D, F16>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, p);
+    if (p.slots) {
+        const dim3 grid((unsigned)(((int64_t)p.T * p.Hq * (D / 4) + 255) / 256));
+        if (c.wide) hipLaunchKernelGGL((scored_merge_kernel<D, kWideRows, F16>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((scored_merge_kernel<D, kFewRows, F16>), grid, dim3(256), 0, st, p);
     }
 }
 
 static int launch_scored(ScoredParams& p, int32_t max_extend_len, int32_t max_seq_len, int32_t D, float scale, float cap, int32_t dtype,
                          void* workspace, int64_t workspace_bytes, void* stream) {
     if (const int e = check_common(p, max_extend_len, max_seq_len, D, scale, cap, dtype)) return e;
-    const ScoredCut c = scored_cut(p.B, p.T, p.Hq, p.Hkv, D, max_extend_len, max_seq_len, p.window);
+    const ScoredCut c = scored_cut(p.B, p.T, p.Hq, p.Hkv, D, max_extend_len, max_seq_len);
     if (c.bytes && (!workspace || workspace_bytes < c.bytes || ((uintptr_t)workspace & 255))) return M355_ERR_WORKSPACE;
-    if ((int64_t)p.B * p.Hkv * c.blocks * c.splits > 0x3fffffffLL || c.splits > 65535 ||
+    if (c.grid > 0x3fffffffLL ||
         (int64_t)p.T * p.Hq * (D / 4) / 256 > 0x3fffffffLL) return M355_ERR_INVALID_ARG;
     p.G = p.Hq / p.Hkv; p.ps_shift = shift_of(p.ps);
     p.scale_log2 = scale * kLog2e; p.cap_log2 = cap * kLog2e; p.cap_rate = cap > 0.f ? 2.f * scale * kLog2e / cap : 0.f;
-    p.blocks = c.blocks; p.splits = c.splits; p.chunk = c.chunk;
-    if (c.bytes) { p.part = (float*)workspace; p.part_n = (int32_t*)((uint8_t*)workspace + c.part_bytes); }
+    p.blocks = c.blocks; p.slots = c.slots; p.max_parts = c.max_parts;
+    if (c.bytes) { p.part = (float*)workspace; p.part_of = (int2*)((uint8_t*)workspace + c.part_bytes); }
     hipStream_t st = (hipStream_t)stream;
     const bool mod = cap > 0.f || p.slopes, f16 = dtype == M355_DTYPE_F16;
 #define M355_SCORED(DD, MM, FF) if (D == DD && mod == MM && f16 == FF) { launch_kernels<DD, MM, FF>(p, c, st); return check_launch(); }
@@ -805,9 +815,9 @@ static int launch_scored(ScoredParams& p, int32_t max_extend_len, int32_t max_se
 using namespace m355;
 
 extern "C" int64_t m355_scored_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_extend_len,
-                                               int32_t max_seq_len_hint, int32_t window) {
-    if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_extend_len <= 0 || max_seq_len_hint <= 0 || window < 0) return 0;
-    return scored_cut(B, T, Hq, Hkv, D, max_extend_len, max_seq_len_hint, window).bytes;
+                                               int32_t max_seq_len_hint) {
+    if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_extend_len <= 0 || max_seq_len_hint <= 0) return 0;
+    return scored_cut(B, T, Hq, Hkv, D, max_extend_len, max_seq_len_hint).bytes;
 }
 
 extern "C" int m355_scored_attn(const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool, int64_t pool_row_stride,

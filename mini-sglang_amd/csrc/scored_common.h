@@ -22,10 +22,11 @@ struct ScoredParams {
     const uint32_t* mask;                                     // trees: [T, words] ancestor bits; null otherwise
     int32_t words;
     const int64_t* positions;                                 // trees: position of every node (read when slopes are given)
-    // the launch: row blocks per request, KV splits per row block and their length in tokens (the last split takes what is left)
-    int32_t blocks, splits, chunk;
-    float* part;                                              // splits > 1: [T * Hq][splits][D + 4] unnormalised O, m, l
-    int32_t* part_n;                                          // [T * Hq] splits that hold a part; 1: the row is already final
+    // the launch: row blocks of the longest request, and - where keys are split - the workgroups that fit the chip at once, the
+    // parts there is room for, and the parts themselves
+    int32_t blocks, slots, max_parts;                         // slots 0: no splits
+    float* part;                                              // [max_parts][rows of a block][D + 4] unnormalised O, m, l
+    int2* part_of;                                            // [T * Hq] {first row of the parts, how many}; 1 and fewer: the row is final
 };
 
 __device__ __forceinline__ ReqSpan load_span(const ScoredParams& p, int b) {
@@ -38,10 +39,116 @@ __device__ __forceinline__ ReqSpan load_span(const ScoredParams& p, int b) {
     return req_span(q0, q1, P, p.seq_lens ? p.seq_lens[b] : P + (q1 - q0), p.T, tokens);
 }
 
+
 __device__ __forceinline__ const int32_t* table_row(const ScoredParams& p, int b) {
     int64_t r = p.page_table_ids[b];
     r = r < 0 ? 0 : (r >= p.pt_rows ? p.pt_rows - 1 : r);
     return p.page_table + r * p.pt_stride;
+}
+
+// One workgroup's share of a call: row block rb of request b, kv head h, part sp of nsp, `chunk` keys each; its rows' results go to
+// part slot part0 + sp.
+struct Share {
+    bool any;
+    int32_t b, h, rb, sp, nsp, chunk, part0;
+    ReqSpan r;
+    const int32_t* pt_row;
+};
+
+// Inclusive sums over the lanes of a wave, in six vector instructions: inside rows of 16, then across them (the sum of lane 15 of
+// each row to the next, of lane 31 to the upper half).
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T dpp_plus(T x) {
+    return x + __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xF, false));
+}
+template <typename T>
+__device__ __forceinline__ T wave_sums(T x) {
+    x = dpp_plus<0x111, 0xF>(x);                       // row_shr:1
+    x = dpp_plus<0x112, 0xF>(x);
+    x = dpp_plus<0x114, 0xF>(x);
+    x = dpp_plus<0x118, 0xF>(x);
+    x = dpp_plus<0x142, 0xA>(x);                       // row_bcast:15
+    return dpp_plus<0x143, 0xC>(x);                    // row_bcast:31
+}
+template <typename T>
+__device__ __forceinline__ T lane_value(T x, int lane) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+}
+
+// Splits follow the batch, which the host does not know: every wave reads the requests' lengths (one per lane) and lays the work
+// out for itself, the same way in all of them.
+//   work  W = sum over requests of row blocks x keys x kv heads; a part holds at most size = W / full_parts keys
+//   parts nsp = ceil(keys / size) per request, all of one length: full_parts + units at most, which sizes grid and workspace
+// Workgroups are numbered request by request, so those with nothing to do come last.  A workgroup that only finds out that it is idle
+// still waits for a place and holds it for 2 us: with idle ones in between, the others started up to 40 us late.
+// Row blocks of one (request, kv head, part) lie 8 apart: on one XCD, whose L2 then reads their keys once.  Their parts come in
+// whole rounds of the 8 XCDs where there are that many (61 to 72 workgroups an XCD instead of 64 cost a second round: 73 us for 58).
+template <int RB, bool FEW>
+__device__ __forceinline__ Share find_share(const ScoredParams& p) {
+    constexpr int32_t shortest_max = FEW ? 128 : 256, shortest_min = FEW ? 128 : 64;     // keys of a part: scored_cut
+    const int lane = threadIdx.x & 63;
+    struct Req { ReqSpan r; int32_t blocks, keys, row; };
+    auto load = [&](int b) {                           // everything a share needs of a request, in one round of loads
+        Req q;
+        const int at = imin(b, p.B - 1);
+        const int64_t row = p.page_table_ids[at];
+        q.r = load_span(p, at);
+        q.row = (int32_t)(row < 0 ? 0 : (row >= p.pt_rows ? p.pt_rows - 1 : row));
+        q.blocks = b < p.B ? (q.r.E * p.G + RB - 1) / RB : 0;
+        q.keys = p.window > 0 ? imin(q.r.L, imin(p.window, 0x3fffffff) + RB) : q.r.L;
+        return q;
+    };
+    const Req first = load(lane);
+    float work = 0.f, units = 0.f;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        const Req q = b0 ? load(b0 + lane) : first;
+        work += lane_value(wave_sums((float)q.blocks * (float)q.keys), 63);
+        units += lane_value(wave_sums((float)q.blocks), 63);
+    }
+    work *= (float)p.Hkv;
+    units *= (float)p.Hkv;
+    const int32_t size = (int32_t)fminf(work / full_parts((float)p.slots, units, FEW), 1e9f) + 1;
+    int32_t at = (int32_t)blockIdx.x, part0 = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        const Req q = b0 ? load(b0 + lane) : first;
+        const int32_t least = imax(size, imax(shortest_min, imin(shortest_max, q.keys / 16)));
+        int32_t nsp = imax(1, (q.keys + least - 1) / least);
+        const bool rounds = q.blocks > 1 && nsp * p.Hkv >= 8;
+        if (rounds) {                                  // the nearest number of parts that gives whole rounds
+            const int32_t step = 8 / imin(p.Hkv & -p.Hkv, 8);
+            nsp = imax(step, (nsp + step / 2) / step * step);
+        }
+        const int32_t items = nsp * p.Hkv * q.blocks, parts = nsp * p.Hkv * q.blocks;
+        const int32_t items_to = wave_sums(items), parts_to = wave_sums(parts);
+        const unsigned long long past = __ballot(at < items_to);
+        if (past) {
+            const int k = __builtin_ctzll(past);       // the request of this workgroup, in lane k
+            const int32_t i = at - lane_value(items_to - items, k), blocks = lane_value(q.blocks, k), n = lane_value(nsp, k);
+            Share s;
+            int32_t u = i;
+            s.rb = 0;
+            if (blocks > 1) {
+                if (n * p.Hkv >= 8) { const int32_t y = i >> 3; s.rb = y % blocks; u = (y / blocks) * 8 + (i & 7); }
+                else { s.rb = i % blocks; u = i / blocks; }
+            }
+            s.any = true;
+            // the kv head turns with part and request: an XCD should not read one head's column of the pools only (8 heads, 8 XCDs)
+            s.sp = u / p.Hkv;
+            s.b = b0 + k;
+            s.h = blocks > 1 ? u % p.Hkv : (u + s.sp + s.b) % p.Hkv;
+            s.nsp = n;
+            s.chunk = ((lane_value(q.keys, k) + n - 1) / n + 63) & ~63;
+            s.part0 = part0 + lane_value(parts_to - parts, k) + (s.rb * p.Hkv + s.h) * n;
+            s.r = {lane_value(q.r.q0, k), lane_value(q.r.E, k), lane_value(q.r.P, k), lane_value(q.r.L, k)};
+            s.pt_row = p.page_table + (int64_t)lane_value(q.row, k) * p.pt_stride;
+            if (s.part0 + n > p.max_parts) s.any = false;              // (only lengths that contradict T get here)
+            return s;
+        }
+        at -= lane_value(items_to, 63);
+        part0 += lane_value(parts_to, 63);
+    }
+    Share none = {};
+    return none;
 }
 
 // Token range of a row block and of the rows' limits inside it: every row of the block sees [lo_max, hi_min), none sees a key

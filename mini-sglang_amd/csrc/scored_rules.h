@@ -54,6 +54,14 @@ M355_HD int32_t pool_slot(int32_t page, int32_t ps, int32_t offset, int64_t S) {
     return (int32_t)s;
 }
 
+// Full parts that `units` units of work are cut into for `slots` workgroups: every unit ends in a part that is half full on average,
+// so the rest would run at once; at least half the slots, where the units alone nearly fill them.  The single-token kernel, which
+// memory alone bounds, keeps a few more places free for workgroups without work.
+M355_HD float full_parts(float slots, float units, bool few) {
+    const float rest = slots - (few ? 0.75f : 0.5f) * units;
+    return rest > 0.5f * slots ? rest : 0.5f * slots;
+}
+
 // A request's rows as the kernels use them: q rows q0 .. q0 + E, positions P + j, L cached tokens - whatever the device
 // arrays hold, every row lies inside the T rows of q and every token inside the table row.
 struct ReqSpan { int32_t q0, E, P, L; };

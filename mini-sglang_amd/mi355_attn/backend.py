@@ -207,7 +207,7 @@ class MI355AttnBackend:
         k_pool, v_pool = batch.kvcache.get_kv_cache(layer.layer_id)
         md = self.forward_metadata
         need = ops.scored_workspace_bytes(batch.seq_lens.numel(), q.shape[0], layer.num_heads, layer.num_kv_heads, layer.head_dim,
-                                          form.get("max_extend_len", 1), md.max_seq_len, mods["window"])
+                                          form.get("max_extend_len", 1), md.max_seq_len)
         return ops.scored_attn(q, k_pool, v_pool, batch.page_manager.page_table, batch.page_table_ids, batch.seq_lens, self.page_size,
                                layer.num_heads, md.max_seq_len, workspace=self._ws(need, q.device), **form, **mods, **masks)
 

@@ -474,8 +474,8 @@ def _scratch(workspace, need: int, device):
 
 
 @functools.lru_cache(maxsize=4096)
-def scored_workspace_bytes(B: int, T: int, Hq: int, Hkv: int, D: int, max_extend_len: int, max_seq_len: int, window: int = 0) -> int:
-    return int(_lib.load().m355_scored_workspace_bytes(B, T, Hq, Hkv, D, max_extend_len, max_seq_len, window))
+def scored_workspace_bytes(B: int, T: int, Hq: int, Hkv: int, D: int, max_extend_len: int, max_seq_len: int) -> int:
+    return int(_lib.load().m355_scored_workspace_bytes(B, T, Hq, Hkv, D, max_extend_len, max_seq_len))
 
 
 def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
@@ -515,7 +515,7 @@ def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, pag
     W = num_heads * D
     q2 = _rows("scored_attn", q, W)
     out, o_stride = _out_rows("scored_attn", q2, out, T, W)
-    need = 0 if workspace is not None else scored_workspace_bytes(B, T, num_heads, Hkv, D, max_extend_len, max_seq_len, window)
+    need = 0 if workspace is not None else scored_workspace_bytes(B, T, num_heads, Hkv, D, max_extend_len, max_seq_len)
     held, ws_ptr, ws_bytes = _scratch(workspace, need, q.device)
     code = _lib.load().m355_scored_attn(q2.data_ptr(), q2.stride(0) if T > 1 else W, k_pool.data_ptr(), v_pool.data_ptr(), pitch, S,
                                         page_table.data_ptr(), pt_stride, pt_rows, pt_cols, ids, lens, pre, cu, out.data_ptr(), o_stride,
