@@ -192,11 +192,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
             bits = row_bits(p, r, t, lo, hi, base);
             const uint32_t w = bits >> (4 * kg);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = (w >> (16 * (i >> 2) + (i & 3))) & 1u ? s[i] : -INFINITY;
-            bool any = false;
+            for (int i = 0; i < 8; ++i) s[i] = masked_score(s[i], w, 16 * (i >> 2) + (i & 3));
+            uint32_t carry = 0;
 #pragma unroll
-            for (int dt = 0; dt < M::DT; ++dt) any = any || frag_nonfinite<F16>(v_frag(st, dt));
-            bad = __any(any);
+            for (int dt = 0; dt < M::DT; ++dt) carry |= frag_carry<F16>(v_frag(st, dt));
+            bad = any_nonfinite(carry);
         }
         float mx = s[0], a, c;
 #pragma unroll
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
 // those of prefill_attn.hip (v_mfma_f32_32x32x16, a lane owns one row and 16 of a tile's keys); what differs is the score
 // stage between them and the range that is walked.
 // ------------------------------------------------------------------------------------------------------------------------
-template <int D, bool MOD, bool F16>
+template <int D, bool MOD, bool F16, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams p) {
     using W = WgCfg<D>;
     constexpr int NW = 4, NBUF = 4;
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     // ---- which rows and keys.  Without splits: all row blocks of one (request, kv head), which walk much the same keys, on one XCD,
     // the last (longest under a causal mask) first; pairs left over after the full rounds of 8 are spread over all XCDs
     Share sh;
-    if (p.slots) {
+    if constexpr (SPLIT) {
         sh = find_share<ROWS, false>(p);
         if (!sh.any) return;
     } else {
@@ -345,7 +345,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     const int row0 = ROWS * tb + 32 * wid, mrow = row0 + c;
     const bool valid = mrow < rows;
     const int j = valid ? mrow / p.G : 0, g = valid ? mrow - j * p.G : 0;
-    const int64_t t = r.q0 + j;
+    const int32_t t = r.q0 + j;
     int32_t pos = r.P + j, lo = 0, hi = r.L;
     BlockRange br = {0x7fffffff, 0, 0, 0x7fffffff};                // the wave's rows
     if (p.mask) {
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     bf16x8 qf[W::KS];
     f32x16 o[W::DT];
     {
-        const uint16_t* qp = p.q + t * p.q_stride + (int64_t)(h * p.G + g) * D + hh * 8;
+        const uint16_t* qp = p.q + (int64_t)t * p.q_stride + (int64_t)(h * p.G + g) * D + hh * 8;
 #pragma unroll
         for (int s = 0; s < W::KS; ++s) {
             u32x4 v = u32x4{0u, 0u, 0u, 0u};
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     const bool none = lo_wg >= hi_wg;
     const int pair0 = none ? 0 : lo_wg >> 6, pairs_end = none ? 0 : (hi_wg + 63) >> 6, n_tiles = (hi_wg + 31) >> 5;
     const int per = sh.chunk >> 6;
-    const int active = imax(1, imin(sh.nsp, (pairs_end - pair0 + per - 1) / per));
+    const int active = SPLIT ? imax(1, imin(sh.nsp, (pairs_end - pair0 + per - 1) / per)) : 1;
     if (sp >= active) return;
     const int p_begin = pair0 + sp * per, n_pairs = sp == active - 1 ? pairs_end : p_begin + per;   // exclusive end
 
@@ -493,7 +493,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     auto mask = [&](f32x16& s, const uint32_t bits) {
         const uint32_t w = bits >> (4 * hh);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = (w >> ((i & 3) + 8 * (i >> 2))) & 1u ? s[i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) s[i] = masked_score(s[i], w, (i & 3) + 8 * (i >> 2));
     };
     float m_run = -INFINITY, l_run = 0.f;
     auto new_max = [&](float mx) {
@@ -534,10 +534,10 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     };
     // infinities and NaN of a tile's V fragments: out of the product, into the rows that see them
     auto clean = [&](bf16x8 (&f)[W::KS], const int buf, const uint32_t bits) {
-        bool any = false;
+        uint32_t carry = 0;
 #pragma unroll
-        for (int s = 0; s < W::KS; ++s) any = any || frag_nonfinite<F16>(f[s]);
-        if (!__any(any)) return;
+        for (int s = 0; s < W::KS; ++s) carry |= frag_carry<F16>(f[s]);
+        if (!any_nonfinite(carry)) return;
 #pragma unroll
         for (int s = 0; s < W::KS; ++s) f[s] = frag_finite<F16>(f[s]);
         for (int tk = 0; tk < 32; ++tk) {
@@ -641,10 +641,10 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     float la, lb;
     lane_pair<32>(l_run, la, lb);
     const float lt = la + lb;
-    const int64_t item = t * p.Hq + h * p.G + g;
+    const int64_t item = (int64_t)t * p.Hq + h * p.G + g;
     if (!valid) return;
     const int prow = 32 * wid + c;                                 // row inside the block
-    if (p.slots && sp == 0 && hh == 0) p.part_of[item] = make_int2(sh.part0 * ROWS + prow, active);
+    if (SPLIT && sp == 0 && hh == 0) p.part_of[item] = make_int2(sh.part0 * ROWS + prow, active);
     if (active > 1) {                                              // unnormalised partial of this split: O^T, m, l
         float* wo = p.part + ((int64_t)(sh.part0 + sp) * ROWS + prow) * (D + 4);
 #pragma unroll
@@ -657,7 +657,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
         return;
     }
     const float inv = 1.f / lt;
-    uint16_t* op = p.out + t * p.o_stride + (int64_t)(h * p.G + g) * D + 4 * hh;
+    uint16_t* op = p.out + (int64_t)t * p.o_stride + (int64_t)(h * p.G + g) * D + 4 * hh;
 #pragma unroll
     for (int dt = 0; dt < W::DT; ++dt)
 #pragma unroll
@@ -779,7 +779,8 @@ static int check_common(const ScoredParams& p, int32_t max_extend_len, int32_t m
 template <int D, bool MOD, bool F16>
 static void launch_kernels(const ScoredParams& p, const ScoredCut& c, hipStream_t st) {
     if (c.wide) {
-        hipLaunchKernelGGL((scored_wide_kernel<D, MOD, F16>), dim3((unsigned)c.grid), dim3(256), 0, st, p);
+        if (p.slots) hipLaunchKernelGGL((scored_wide_kernel<D, MOD, F16, true>), dim3((unsigned)c.grid), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((scored_wide_kernel<D, MOD, F16, false>), dim3((unsigned)c.grid), dim3(256), 0, st, p);
     } else {
         hipLaunchKernelGGL((scored_few_kernel<D, MOD, F16>), dim3((unsigned)c.grid), dim3(64 * kFewWaves), 0, st, p);
     }

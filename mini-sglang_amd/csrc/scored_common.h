@@ -175,34 +175,39 @@ __device__ __forceinline__ float cap_score(const ScoredParams& p, float s) {
     return fmaf(-2.f * p.cap_log2, __builtin_amdgcn_rcpf(1.f + exp2_fast(s * p.cap_rate)), p.cap_log2);
 }
 
-// Two 16-bit values of a dword: does one of them have all exponent bits set (infinity or NaN), and the dword without those
+// Infinities and NaN among the two 16-bit values of a dword: all exponent bits set.  Adding one to the exponent field then carries into
+// the half's top bit, and only then - whole numbers without a compare, of which a tile needs hundreds at once.
 template <bool F16>
-__device__ __forceinline__ bool has_nonfinite(uint32_t w) {
-    constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;
-    return (w & e) == e || ((w >> 16) & e) == e;
+__device__ __forceinline__ uint32_t exponent_carry(uint32_t w) {
+    constexpr uint32_t field = F16 ? 0x7c007c00u : 0x7f807f80u, one = F16 ? 0x04000400u : 0x00800080u;
+    return (w & field) + one;                          // bit 15 / 31: that half is not finite
 }
 template <bool F16>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
-    constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;
-    if ((w & e) == e) w &= 0xffff0000u;
-    if (((w >> 16) & e) == e) w &= 0x0000ffffu;
-    return w;
-}
+__device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) { return ((exponent_carry<F16>(w) >> 15) & 0x00010001u) * 0xffffu; }
 template <bool F16>
-__device__ __forceinline__ bool frag_nonfinite(bf16x8 f) {
+__device__ __forceinline__ uint32_t frag_carry(bf16x8 f) {
     const u32x4 w = __builtin_bit_cast(u32x4, f);
-    return has_nonfinite<F16>(w[0]) || has_nonfinite<F16>(w[1]) || has_nonfinite<F16>(w[2]) || has_nonfinite<F16>(w[3]);
+    return exponent_carry<F16>(w[0]) | exponent_carry<F16>(w[1]) | exponent_carry<F16>(w[2]) | exponent_carry<F16>(w[3]);
 }
+__device__ __forceinline__ bool any_nonfinite(uint32_t carry) { return __any((carry & 0x80008000u) != 0); }
 template <bool F16>
 __device__ __forceinline__ bf16x8 frag_finite(bf16x8 f) {
-    const u32x4 w = __builtin_bit_cast(u32x4, f);
-    return __builtin_bit_cast(bf16x8, u32x4{finite_only<F16>(w[0]), finite_only<F16>(w[1]), finite_only<F16>(w[2]), finite_only<F16>(w[3])});
+    u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] &= ~nonfinite_halves<F16>(w[i]);
+    return __builtin_bit_cast(bf16x8, w);
 }
 // the infinities and NaN of four consecutive values, 0 for the others
 template <bool F16>
 __device__ __forceinline__ f32x4 nonfinite4(uint2 w) {
-    const uint32_t x = w.x & ~finite_only<F16>(w.x), y = w.y & ~finite_only<F16>(w.y);
+    const uint32_t x = w.x & nonfinite_halves<F16>(w.x), y = w.y & nonfinite_halves<F16>(w.y);
     return f32x4{unpack16_lo<F16>(x), unpack16_hi<F16>(x), unpack16_lo<F16>(y), unpack16_hi<F16>(y)};
+}
+
+// s where bit `bit` of `seen` is set, -inf elsewhere
+__device__ __forceinline__ float masked_score(float s, uint32_t seen, int bit) {
+    const uint32_t keep = (uint32_t)((int32_t)(seen << (31 - bit)) >> 31);
+    return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, s) & keep) | (0xff800000u & ~keep));
 }
 
 __device__ __forceinline__ int32_t slot_of(const ScoredParams& p, const int32_t* pt_row, int32_t tok) {
