@@ -251,28 +251,44 @@ int m355_rope_kv_store(void *q, int64_t q_row_stride, void *k, int64_t k_row_str
  *     x_k = scale * q[t,h] . K[k];   x_k = softcap * tanh(x_k / softcap)  (softcap > 0);
  *     x_k -= slopes[h] * |pos - k|   (slopes != NULL, fp32 [Hq]);
  *     out[t, h, :] = sum_k softmax(x)_k V[k, h / (Hq/Hkv), :]
- * Visible keys: lo <= k < hi, lo = max(0, doc_starts[t], window > 0 ? pos - window + 1 : 0),
+ * m355_scored_attn: visible keys lo <= k < hi, lo = max(0, doc_starts[t], window > 0 ? pos - window + 1 : 0),
  * hi = min(seq_lens[b], max(pos + 1, bidir_lens[b])).  doc_starts int32 [T] (first position of the row's document),
- * bidir_lens int32 [B] (a prompt prefix of that many tokens that is visible to every row of the request); NULL: none.  A row
- * that sees nothing - its mask is empty, or every visible score is -inf - gives zeros.  What masked keys and values hold
- * never reaches an output, infinities and NaN included.
+ * bidir_lens int32 [B] (a prompt prefix of that many tokens that is visible to every row of the request); NULL: none.
  * Two forms: prefix_lens / cu_q given - row cu_q[b] + j is the token at position prefix_lens[b] + j, as m355_prefill_attn
  * (rows at or past cu_q[B] are left alone); both NULL - one row per request, its newest token at seq_lens[b] - 1 (a request of
- * length 0 gives zeros).  Any Hq that is a multiple of Hkv; head_dim 64 or 128; bf16 or fp16.
- * S = token rows of the pools (< 2^31); pt_rows / pt_cols = the table's shape.  Whatever the tables hold, nothing outside the
- * pools, the table and the T rows is read: ids and pages out of range are brought back into it.
- * max_extend_len >= the longest cu_q[b+1] - cu_q[b] (rows past it are not computed); max_seq_len_hint >= the longest
- * request, for the choice of the launch.  workspace: m355_scored_workspace_bytes bytes (the same sizes), 256-byte aligned, may be
- * NULL where that is 0; calls that overlap need one each. */
+ * length 0 gives zeros).
+ * m355_tree_attn: row cu_q[b] + j is node j of request b's draft tree (m355_tree_prepare); it sees the prefix_lens[b] cached tokens
+ * and the nodes of its mask row, whose K/V are in the pools already.  Distances between nodes are differences of depth: positions is
+ * read for the bias only and may be NULL without slopes.  seq_lens, window, doc_starts and bidir_lens must be NULL / 0.
+ * A row that sees nothing - its mask is empty, or every visible score is -inf - gives zeros.  What masked keys and values hold
+ * never reaches an output, infinities and NaN included.  Any Hq that is a multiple of Hkv; head_dim 64 or 128; bf16 or fp16.
+ * Whatever the tables hold, nothing outside the pools, the table and the T rows is read: ids and pages out of range are brought
+ * back into it.  out must not overlap q. */
+typedef struct M355ScoredArgs {
+    const void *q, *k_pool, *v_pool; /* [T, Hq*D], [pool_rows, Hkv, D] twice                              */
+    const int32_t *page_table;       /* [pt_rows, pt_cols]                                                */
+    const int64_t *page_table_ids, *seq_lens, *prefix_lens; /* [B]                                        */
+    const int32_t *cu_q;             /* [B+1]                                                             */
+    void *out;                       /* [T, Hq*D]                                                         */
+    const float *slopes;
+    const int32_t *doc_starts, *bidir_lens;
+    const uint32_t *tree_mask;       /* [T, mask_words]                                                   */
+    const int64_t *positions;        /* [T]                                                               */
+    void *workspace;                 /* m355_scored_workspace_bytes bytes, 256-byte aligned, may be NULL where that is 0;
+                                        calls that overlap need one each                                  */
+    int64_t q_row_stride, o_row_stride;
+    int64_t pool_row_stride, pool_rows; /* 0: contiguous;  token rows of the pools, < 2^31                */
+    int64_t pt_row_stride, workspace_bytes;
+    int32_t pt_rows, pt_cols, B, T;
+    int32_t max_extend_len;          /* >= the longest cu_q[b+1] - cu_q[b]: rows past it may be left out  */
+    int32_t max_seq_len_hint;        /* >= the longest request, for the choice of the launch              */
+    int32_t Hq, Hkv, D, page_size, window, mask_words, dtype;
+    float scale, softcap;
+} M355ScoredArgs;
 int64_t m355_scored_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_extend_len,
                                     int32_t max_seq_len_hint);
-int m355_scored_attn(const void *q, int64_t q_row_stride, const void *k_pool, const void *v_pool, int64_t pool_row_stride,
-                     int64_t S, const int32_t *page_table, int64_t pt_row_stride, int32_t pt_rows, int32_t pt_cols,
-                     const int64_t *page_table_ids, const int64_t *seq_lens, const int64_t *prefix_lens, const int32_t *cu_q,
-                     void *out, int64_t o_row_stride, int32_t B, int32_t T, int32_t max_extend_len, int32_t max_seq_len_hint,
-                     int32_t Hq, int32_t Hkv, int32_t D, int32_t page_size, float scale, float softcap, const float *slopes,
-                     int32_t window, const int32_t *doc_starts, const int32_t *bidir_lens, void *workspace,
-                     int64_t workspace_bytes, int32_t dtype, void *stream);
+int m355_scored_attn(const M355ScoredArgs *args, void *stream);
+int m355_tree_attn(const M355ScoredArgs *args, void *stream);
 
 /* Trees of drafted tokens (speculative decoding; no counterpart in the reference).  Request b holds prefix_lens[b] cached
  * tokens and brings cu_q[b+1] - cu_q[b] nodes (at most max_nodes <= M355_TREE_MAX_NODES); parents[cu_q[b] + j] is the index of
@@ -288,16 +304,6 @@ int m355_tree_prepare(int32_t *page_table, int64_t pt_row_stride, int32_t pt_row
                       const int64_t *prefix_lens, const int32_t *parents, const int32_t *cu_q, const int32_t *new_pages,
                       const int32_t *new_page_off, int32_t B, int32_t T, int32_t max_nodes, int32_t page_size,
                       uint32_t *tree_mask, int32_t mask_words, int64_t *positions, int64_t *out_cache_loc, void *stream);
-
-/* Attention of the trees' nodes: node t sees the request's prefix_lens[b] cached tokens and the nodes of its mask row (their
- * K/V already in the pools).  Scores, zeros, bounds, workspace (m355_scored_workspace_bytes with max_extend_len = max_nodes) as m355_scored_attn; max_seq_len_hint >= the longest prefix + nodes; positions is read for the bias only
- * (distance = difference of depths) and may be NULL without slopes. */
-int m355_tree_attn(const void *q, int64_t q_row_stride, const void *k_pool, const void *v_pool, int64_t pool_row_stride, int64_t S,
-                   const int32_t *page_table, int64_t pt_row_stride, int32_t pt_rows, int32_t pt_cols,
-                   const int64_t *page_table_ids, const int64_t *prefix_lens, const int32_t *cu_q, const uint32_t *tree_mask,
-                   int32_t mask_words, const int64_t *positions, void *out, int64_t o_row_stride, int32_t B, int32_t T,
-                   int32_t max_nodes, int32_t max_seq_len_hint, int32_t Hq, int32_t Hkv, int32_t D, int32_t page_size, float scale,
-                   float softcap, const float *slopes, void *workspace, int64_t workspace_bytes, int32_t dtype, void *stream);
 
 /* Log probabilities of given tokens, entropy and top alternatives (the reference's sampler, layers/sampler.py:19-29, keeps
  * none).  Per row of logits [T, V] (bf16, fp16 or fp32; any row stride >= V, no alignment beyond the element's), with

@@ -762,17 +762,18 @@ static ScoredCut scored_cut(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int32
 }
 
 // what both entry points refuse
-static int check_common(const ScoredParams& p, int32_t max_extend_len, int32_t max_seq_len, int32_t D, float scale, float cap, int32_t dtype) {
-    if (!p.q || !p.k_pool || !p.v_pool || !p.page_table || !p.page_table_ids || !p.out) return M355_ERR_INVALID_ARG;
-    if (p.B < 0 || p.T < 0 || p.Hq <= 0 || p.Hkv <= 0 || p.Hq % p.Hkv || p.ps <= 0 || p.pt_rows <= 0 || p.pt_cols <= 0) return M355_ERR_INVALID_ARG;
-    if (p.S <= 0 || p.S > 0x7fffffffLL || p.pt_stride < p.pt_cols || (int64_t)p.pt_cols * p.ps > 0x3fffffffLL) return M355_ERR_INVALID_ARG;
-    if (max_extend_len <= 0 || max_seq_len <= 0 || p.window < 0) return M355_ERR_INVALID_ARG;
-    if (!(scale > 0.f) || !(scale < 1e30f) || !(cap >= 0.f) || !(cap < 1e30f)) return M355_ERR_INVALID_ARG;
-    if (dtype != M355_DTYPE_BF16 && dtype != M355_DTYPE_F16) return M355_ERR_UNSUPPORTED;
-    if (D != 64 && D != 128) return M355_ERR_UNSUPPORTED;
-    if (p.row_elems < (int64_t)p.Hkv * D || p.row_elems % 8) return M355_ERR_INVALID_ARG;
-    if (((uintptr_t)p.q | (uintptr_t)p.k_pool | (uintptr_t)p.v_pool | (uintptr_t)p.out) & 15) return M355_ERR_INVALID_ARG;
-    if (p.q_stride % 8 || p.o_stride % 8 || p.q_stride < (int64_t)p.Hq * D || p.o_stride < (int64_t)p.Hq * D) return M355_ERR_INVALID_ARG;
+static int check_args(const M355ScoredArgs& a) {
+    if (!a.q || !a.k_pool || !a.v_pool || !a.page_table || !a.page_table_ids || !a.out) return M355_ERR_INVALID_ARG;
+    if (a.B < 0 || a.T < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.Hq % a.Hkv || a.page_size <= 0 || a.pt_rows <= 0 || a.pt_cols <= 0) return M355_ERR_INVALID_ARG;
+    if (a.pool_rows <= 0 || a.pool_rows > 0x7fffffffLL || a.pt_row_stride < a.pt_cols || (int64_t)a.pt_cols * a.page_size > 0x3fffffffLL) return M355_ERR_INVALID_ARG;
+    if (a.max_extend_len <= 0 || a.max_seq_len_hint <= 0 || a.window < 0) return M355_ERR_INVALID_ARG;
+    if (!(a.scale > 0.f) || !(a.scale < 1e30f) || !(a.softcap >= 0.f) || !(a.softcap < 1e30f)) return M355_ERR_INVALID_ARG;
+    if (a.dtype != M355_DTYPE_BF16 && a.dtype != M355_DTYPE_F16) return M355_ERR_UNSUPPORTED;
+    if (a.D != 64 && a.D != 128) return M355_ERR_UNSUPPORTED;
+    const int64_t W = (int64_t)a.Hq * a.D, row = a.pool_row_stride ? a.pool_row_stride : (int64_t)a.Hkv * a.D;
+    if (row < (int64_t)a.Hkv * a.D || row % 8) return M355_ERR_INVALID_ARG;
+    if (((uintptr_t)a.q | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool | (uintptr_t)a.out) & 15) return M355_ERR_INVALID_ARG;
+    if (a.q_row_stride % 8 || a.o_row_stride % 8 || a.q_row_stride < W || a.o_row_stride < W) return M355_ERR_INVALID_ARG;
     return M355_OK;
 }
 
@@ -791,20 +792,27 @@ static void launch_kernels(const ScoredParams& p, const ScoredCut& c, hipStream_
     }
 }
 
-static int launch_scored(ScoredParams& p, int32_t max_extend_len, int32_t max_seq_len, int32_t D, float scale, float cap, int32_t dtype,
-                         void* workspace, int64_t workspace_bytes, void* stream) {
-    if (const int e = check_common(p, max_extend_len, max_seq_len, D, scale, cap, dtype)) return e;
-    const ScoredCut c = scored_cut(p.B, p.T, p.Hq, p.Hkv, D, max_extend_len, max_seq_len);
-    if (c.bytes && (!workspace || workspace_bytes < c.bytes || ((uintptr_t)workspace & 255))) return M355_ERR_WORKSPACE;
-    if (c.grid > 0x3fffffffLL ||
-        (int64_t)p.T * p.Hq * (D / 4) / 256 > 0x3fffffffLL) return M355_ERR_INVALID_ARG;
-    p.G = p.Hq / p.Hkv; p.ps_shift = shift_of(p.ps);
-    p.scale_log2 = scale * kLog2e; p.cap_log2 = cap * kLog2e; p.cap_rate = cap > 0.f ? 2.f * scale * kLog2e / cap : 0.f;
+static int launch_scored(const M355ScoredArgs& a, void* stream) {
+    if (const int e = check_args(a)) return e;
+    const int32_t ext = a.cu_q ? a.max_extend_len : 1;
+    const ScoredCut c = scored_cut(a.B, a.T, a.Hq, a.Hkv, a.D, ext, a.max_seq_len_hint);
+    if (c.bytes && (!a.workspace || a.workspace_bytes < c.bytes || ((uintptr_t)a.workspace & 255))) return M355_ERR_WORKSPACE;
+    if (c.grid > 0x3fffffffLL || (int64_t)a.T * a.Hq * (a.D / 4) / 256 > 0x3fffffffLL) return M355_ERR_INVALID_ARG;
+    ScoredParams p = {};
+    p.q = (const uint16_t*)a.q; p.k_pool = (const uint16_t*)a.k_pool; p.v_pool = (const uint16_t*)a.v_pool;
+    p.page_table = a.page_table; p.page_table_ids = a.page_table_ids; p.seq_lens = a.seq_lens; p.prefix_lens = a.prefix_lens; p.cu_q = a.cu_q;
+    p.out = (uint16_t*)a.out; p.q_stride = a.q_row_stride; p.o_stride = a.o_row_stride;
+    p.row_elems = a.pool_row_stride ? a.pool_row_stride : (int64_t)a.Hkv * a.D;
+    p.pt_stride = a.pt_row_stride; p.S = a.pool_rows; p.pt_rows = a.pt_rows; p.pt_cols = a.pt_cols;
+    p.B = a.B; p.T = a.T; p.Hq = a.Hq; p.Hkv = a.Hkv; p.G = a.Hq / a.Hkv; p.ps = a.page_size; p.ps_shift = shift_of(a.page_size);
+    p.scale_log2 = a.scale * kLog2e; p.cap_log2 = a.softcap * kLog2e; p.cap_rate = a.softcap > 0.f ? 2.f * a.scale * kLog2e / a.softcap : 0.f;
+    p.slopes = a.slopes; p.window = a.window; p.doc_starts = a.doc_starts; p.bidir = a.bidir_lens;
+    p.mask = a.tree_mask; p.words = a.mask_words; p.positions = a.positions;
     p.blocks = c.blocks; p.slots = c.slots; p.max_parts = c.max_parts;
-    if (c.bytes) { p.part = (float*)workspace; p.part_of = (int2*)((uint8_t*)workspace + c.part_bytes); }
+    if (c.bytes) { p.part = (float*)a.workspace; p.part_of = (int2*)((uint8_t*)a.workspace + c.part_bytes); }
     hipStream_t st = (hipStream_t)stream;
-    const bool mod = cap > 0.f || p.slopes, f16 = dtype == M355_DTYPE_F16;
-#define M355_SCORED(DD, MM, FF) if (D == DD && mod == MM && f16 == FF) { launch_kernels<DD, MM, FF>(p, c, st); return check_launch(); }
+    const bool mod = a.softcap > 0.f || a.slopes, f16 = a.dtype == M355_DTYPE_F16;
+#define M355_SCORED(DD, MM, FF) if (a.D == DD && mod == MM && f16 == FF) { launch_kernels<DD, MM, FF>(p, c, st); return check_launch(); }
     M355_SCORED(64, false, false) M355_SCORED(64, false, true) M355_SCORED(64, true, false) M355_SCORED(64, true, true)
     M355_SCORED(128, false, false) M355_SCORED(128, false, true) M355_SCORED(128, true, false) M355_SCORED(128, true, true)
 #undef M355_SCORED
@@ -821,41 +829,20 @@ extern "C" int64_t m355_scored_workspace_bytes(int32_t B, int32_t T, int32_t Hq,
     return scored_cut(B, T, Hq, Hkv, D, max_extend_len, max_seq_len_hint).bytes;
 }
 
-extern "C" int m355_scored_attn(const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool, int64_t pool_row_stride,
-                                int64_t S, const int32_t* page_table, int64_t pt_row_stride, int32_t pt_rows, int32_t pt_cols,
-                                const int64_t* page_table_ids, const int64_t* seq_lens, const int64_t* prefix_lens,
-                                const int32_t* cu_q, void* out, int64_t o_row_stride, int32_t B, int32_t T, int32_t max_extend_len,
-                                int32_t max_seq_len_hint, int32_t Hq, int32_t Hkv, int32_t D, int32_t page_size, float scale,
-                                float softcap, const float* slopes, int32_t window, const int32_t* doc_starts,
-                                const int32_t* bidir_lens, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream) {
-    if (T == 0 || B == 0) return M355_OK;
-    if (!seq_lens || (prefix_lens == nullptr) != (cu_q == nullptr) || (!cu_q && T < B)) return M355_ERR_INVALID_ARG;
-    ScoredParams p = {};
-    p.q = (const uint16_t*)q; p.k_pool = (const uint16_t*)k_pool; p.v_pool = (const uint16_t*)v_pool;
-    p.page_table = page_table; p.page_table_ids = page_table_ids; p.seq_lens = seq_lens; p.prefix_lens = prefix_lens; p.cu_q = cu_q;
-    p.out = (uint16_t*)out; p.q_stride = q_row_stride; p.o_stride = o_row_stride;
-    p.row_elems = pool_row_stride ? pool_row_stride : (int64_t)Hkv * D;
-    p.pt_stride = pt_row_stride; p.S = S; p.pt_rows = pt_rows; p.pt_cols = pt_cols; p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv;
-    p.ps = page_size; p.slopes = slopes; p.window = window; p.doc_starts = doc_starts; p.bidir = bidir_lens;
-    return launch_scored(p, cu_q ? max_extend_len : 1, max_seq_len_hint, D, scale, softcap, dtype, workspace, workspace_bytes, stream);
+extern "C" int m355_scored_attn(const M355ScoredArgs* args, void* stream) {
+    if (!args) return M355_ERR_INVALID_ARG;
+    const M355ScoredArgs& a = *args;
+    if (a.T == 0 || a.B == 0) return M355_OK;
+    if (!a.seq_lens || a.tree_mask || a.mask_words || (a.prefix_lens == nullptr) != (a.cu_q == nullptr)) return M355_ERR_INVALID_ARG;
+    if (!a.cu_q && a.T < a.B) return M355_ERR_INVALID_ARG;
+    return launch_scored(a, stream);
 }
 
-extern "C" int m355_tree_attn(const void* q, int64_t q_row_stride, const void* k_pool, const void* v_pool, int64_t pool_row_stride,
-                              int64_t S, const int32_t* page_table, int64_t pt_row_stride, int32_t pt_rows, int32_t pt_cols,
-                              const int64_t* page_table_ids, const int64_t* prefix_lens, const int32_t* cu_q,
-                              const uint32_t* tree_mask, int32_t mask_words, const int64_t* positions, void* out, int64_t o_row_stride,
-                              int32_t B, int32_t T, int32_t max_nodes, int32_t max_seq_len_hint, int32_t Hq, int32_t Hkv, int32_t D,
-                              int32_t page_size, float scale, float softcap, const float* slopes, void* workspace,
-                              int64_t workspace_bytes, int32_t dtype, void* stream) {
-    if (T == 0 || B == 0) return M355_OK;
-    if (!prefix_lens || !cu_q || !tree_mask || mask_words <= 0 || (slopes && !positions)) return M355_ERR_INVALID_ARG;
-    if ((int64_t)mask_words * 32 < max_nodes) return M355_ERR_INVALID_ARG;
-    ScoredParams p = {};
-    p.q = (const uint16_t*)q; p.k_pool = (const uint16_t*)k_pool; p.v_pool = (const uint16_t*)v_pool;
-    p.page_table = page_table; p.page_table_ids = page_table_ids; p.prefix_lens = prefix_lens; p.cu_q = cu_q;
-    p.out = (uint16_t*)out; p.q_stride = q_row_stride; p.o_stride = o_row_stride;
-    p.row_elems = pool_row_stride ? pool_row_stride : (int64_t)Hkv * D;
-    p.pt_stride = pt_row_stride; p.S = S; p.pt_rows = pt_rows; p.pt_cols = pt_cols; p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv;
-    p.ps = page_size; p.slopes = slopes; p.mask = tree_mask; p.words = mask_words; p.positions = positions;
-    return launch_scored(p, max_nodes, max_seq_len_hint, D, scale, softcap, dtype, workspace, workspace_bytes, stream);
+extern "C" int m355_tree_attn(const M355ScoredArgs* args, void* stream) {
+    if (!args) return M355_ERR_INVALID_ARG;
+    const M355ScoredArgs& a = *args;
+    if (a.T == 0 || a.B == 0) return M355_OK;
+    if (!a.prefix_lens || !a.cu_q || !a.tree_mask || a.mask_words <= 0 || (int64_t)a.mask_words * 32 < a.max_extend_len) return M355_ERR_INVALID_ARG;
+    if (a.seq_lens || a.window || a.doc_starts || a.bidir_lens || (a.slopes && !a.positions)) return M355_ERR_INVALID_ARG;
+    return launch_scored(a, stream);
 }

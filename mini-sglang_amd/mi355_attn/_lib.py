@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_uint32, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -30,6 +31,14 @@ class OprojRank(ctypes.Structure):   # M355OprojRank (include/mi355tp.h)
     _fields_ = [("x", c_void_p), ("x_row_stride", c_int64), ("w", c_void_p), ("w_row_stride", c_int64),
                 ("out", c_void_p), ("out_row_stride", c_int64), ("recv", c_void_p * MAX_RANKS),
                 ("flags", c_void_p * MAX_RANKS), ("rank", c_int32), ("reserved", c_int32)]
+
+
+# M355ScoredArgs (include/mi355attn.h), packed in one step: filling a ctypes structure field by field costs more than the launch
+SCORED_ARGS = struct.Struct("@15P6q13i2f4x")
+SCORED_FIELDS = ("q", "k_pool", "v_pool", "page_table", "page_table_ids", "seq_lens", "prefix_lens", "cu_q", "out", "slopes", "doc_starts",
+                 "bidir_lens", "tree_mask", "positions", "workspace", "q_row_stride", "o_row_stride", "pool_row_stride", "pool_rows",
+                 "pt_row_stride", "workspace_bytes", "pt_rows", "pt_cols", "B", "T", "max_extend_len", "max_seq_len_hint", "Hq", "Hkv", "D",
+                 "page_size", "window", "mask_words", "dtype", "scale", "softcap")
 
 
 # name -> (restype, argtypes); must list every symbol include/mi355attn.h and include/mi355tp.h declare
@@ -84,16 +93,10 @@ SIGNATURES = {
                                      c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int32, c_int32,
                                      c_int64, c_int32, c_void_p]),
     "m355_scored_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
-    "m355_scored_attn": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int32, c_int32,
-                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32,
-                                   c_int32, c_int32, c_int32, c_int32, c_float, c_float, c_void_p, c_int32, c_void_p, c_void_p,
-                                   c_void_p, c_int64, c_int32, c_void_p]),
+    "m355_scored_attn": (c_int32, [c_char_p, c_void_p]),        # M355ScoredArgs, packed (SCORED_ARGS)
+    "m355_tree_attn": (c_int32, [c_char_p, c_void_p]),
     "m355_tree_prepare": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                     c_int32, c_int32, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
-    "m355_tree_attn": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int32, c_int32,
-                                 c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int32, c_int32,
-                                 c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_float, c_void_p, c_void_p, c_int64,
-                                 c_int32, c_void_p]),
     "m355_token_logprobs_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32]),
     "m355_token_logprobs": (c_int32, [c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p,
                                       c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p]),

@@ -465,7 +465,7 @@ def _scratch(workspace, need: int, device):
     """(tensor that owns it, address, bytes) of a call's workspace: the caller's, or a new one of `need` bytes."""
     if workspace is None:
         if not need:
-            return None, None, 0
+            return None, 0, 0
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
         return workspace, workspace.data_ptr(), need
     if not workspace.is_contiguous():
@@ -500,7 +500,7 @@ def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, pag
     S, Hkv, D, pitch = _pools("scored_attn", q, k_pool, v_pool)
     pt_rows, pt_cols, pt_stride = _table("scored_attn", page_table, page_size)
     lens, ids = _vector("seq_lens", seq_lens, torch.int64, B), _vector("page_table_ids", page_table_ids, torch.int64, B)
-    pre = cu = None
+    pre = cu = 0
     if cu_q is not None and prefix_lens is not None:
         pre, cu = _vector("prefix_lens", prefix_lens, torch.int64, B), _vector("cu_q", cu_q, torch.int32, B + 1)
     elif cu_q is not None or prefix_lens is not None:
@@ -509,19 +509,19 @@ def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, pag
         max_extend_len = 1
         if T != B:
             raise _lib.MI355AttnError(f"scored_attn: {T} rows for {B} requests (pass prefix_lens and cu_q for more than one row each)")
-    slope_ptr = None if slopes is None else _vector("slopes", slopes, torch.float32, num_heads)
-    doc_ptr = None if doc_starts is None else _vector("doc_starts", doc_starts, torch.int32, T)
-    bidir_ptr = None if bidir_lens is None else _vector("bidir_lens", bidir_lens, torch.int32, B)
+    slope_ptr = 0 if slopes is None else _vector("slopes", slopes, torch.float32, num_heads)
+    doc_ptr = 0 if doc_starts is None else _vector("doc_starts", doc_starts, torch.int32, T)
+    bidir_ptr = 0 if bidir_lens is None else _vector("bidir_lens", bidir_lens, torch.int32, B)
     W = num_heads * D
     q2 = _rows("scored_attn", q, W)
     out, o_stride = _out_rows("scored_attn", q2, out, T, W)
     need = 0 if workspace is not None else scored_workspace_bytes(B, T, num_heads, Hkv, D, max_extend_len, max_seq_len)
     held, ws_ptr, ws_bytes = _scratch(workspace, need, q.device)
-    code = _lib.load().m355_scored_attn(q2.data_ptr(), q2.stride(0) if T > 1 else W, k_pool.data_ptr(), v_pool.data_ptr(), pitch, S,
-                                        page_table.data_ptr(), pt_stride, pt_rows, pt_cols, ids, lens, pre, cu, out.data_ptr(), o_stride,
-                                        B, T, max_extend_len, max_seq_len, num_heads, Hkv, D, page_size,
-                                        D ** -0.5 if scale is None else scale, softcap, slope_ptr, window, doc_ptr, bidir_ptr, ws_ptr,
-                                        ws_bytes, dtype_code(q.dtype), current_stream())
+    code = _lib.load().m355_scored_attn(
+        _lib.SCORED_ARGS.pack(q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ids, lens, pre, cu, out.data_ptr(),
+                              slope_ptr, doc_ptr, bidir_ptr, 0, 0, ws_ptr, q2.stride(0) if T > 1 else W, o_stride, pitch, S, pt_stride, ws_bytes,
+                              pt_rows, pt_cols, B, T, max_extend_len, max_seq_len, num_heads, Hkv, D, page_size, window, 0,
+                              dtype_code(q.dtype), D ** -0.5 if scale is None else scale, softcap), current_stream())
     if code:
         check(code, "m355_scored_attn")
     return out
@@ -588,17 +588,17 @@ def tree_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_
     cu, pos_ptr = _vector("plan.cu_q", cu_q, torch.int32, B + 1), _vector("plan.positions", positions, torch.int64, T)
     if mask.dtype is not torch.int32 or mask.dim() != 2 or mask.shape[0] != T or not mask.is_contiguous():
         raise _lib.MI355AttnError(f"tree_attn: the plan is for {mask.shape[0]} nodes, q has {T} rows")
-    slope_ptr = None if slopes is None else _vector("slopes", slopes, torch.float32, num_heads)
+    slope_ptr = 0 if slopes is None else _vector("slopes", slopes, torch.float32, num_heads)
     W = num_heads * D
     q2 = _rows("tree_attn", q, W)
     out, o_stride = _out_rows("tree_attn", q2, out, T, W)
     need = 0 if workspace is not None else scored_workspace_bytes(B, T, num_heads, Hkv, D, plan.max_nodes, max_seq_len)
     held, ws_ptr, ws_bytes = _scratch(workspace, need, q.device)
-    code = _lib.load().m355_tree_attn(q2.data_ptr(), q2.stride(0) if T > 1 else W, k_pool.data_ptr(), v_pool.data_ptr(), pitch, S,
-                                      page_table.data_ptr(), pt_stride, pt_rows, pt_cols, ids, pre, cu, mask.data_ptr(), mask.shape[1], pos_ptr,
-                                      out.data_ptr(), o_stride, B, T, plan.max_nodes, max_seq_len, num_heads, Hkv, D, page_size,
-                                      D ** -0.5 if scale is None else scale, softcap, slope_ptr, ws_ptr, ws_bytes, dtype_code(q.dtype),
-                                      current_stream())
+    code = _lib.load().m355_tree_attn(
+        _lib.SCORED_ARGS.pack(q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ids, 0, pre, cu, out.data_ptr(),
+                              slope_ptr, 0, 0, mask.data_ptr(), pos_ptr, ws_ptr, q2.stride(0) if T > 1 else W, o_stride, pitch, S, pt_stride,
+                              ws_bytes, pt_rows, pt_cols, B, T, plan.max_nodes, max_seq_len, num_heads, Hkv, D, page_size, 0, mask.shape[1],
+                              dtype_code(q.dtype), D ** -0.5 if scale is None else scale, softcap), current_stream())
     if code:
         check(code, "m355_tree_attn")
     return out

@@ -91,48 +91,79 @@ def test_inconsistent_batches_stay_inside_q(rules):
 A16 = 0x10000                                            # an aligned address that is never followed: the calls return first
 
 
+def _pack(base, kw):
+    from mi355_attn import _lib
+    a = {**dict.fromkeys(_lib.SCORED_FIELDS, 0), **base, **kw}
+    assert set(a) == set(_lib.SCORED_FIELDS)
+    return _lib.SCORED_ARGS.pack(*(a[n] or 0 for n in _lib.SCORED_FIELDS))
+
+
+_BOTH = dict(q=A16, q_row_stride=512, k_pool=A16, v_pool=A16, pool_rows=64, page_table=A16, pt_row_stride=8, pt_rows=4, pt_cols=8,
+             page_table_ids=A16, out=A16, o_row_stride=512, B=2, max_seq_len_hint=100, Hq=8, Hkv=2, D=64, page_size=16, scale=0.125)
+
+
 def _scored_args(**kw):
-    a = dict(q=A16, qs=512, k=A16, v=A16, pool=0, S=64, pt=A16, pts=8, rows=4, cols=8, ids=A16, lens=A16, pre=None, cu=None, out=A16,
-             os=512, B=2, T=2, ext=1, mx=100, Hq=8, Hkv=2, D=64, ps=16, scale=0.125, cap=0.0, slopes=None, win=0, doc=None, bi=None,
-             ws=None, wsb=0, dt=0, st=None)
-    assert not set(kw) - set(a)
-    return list({**a, **kw}.values())
+    return _pack(dict(_BOTH, seq_lens=A16, T=2, max_extend_len=1), kw)
 
 
 def _tree_args(**kw):
-    a = dict(q=A16, qs=512, k=A16, v=A16, pool=0, S=64, pt=A16, pts=8, rows=4, cols=8, ids=A16, pre=A16, cu=A16, mask=A16, words=1,
-             pos=None, out=A16, os=512, B=2, T=9, nodes=8, mx=100, Hq=8, Hkv=2, D=64, ps=16, scale=0.125, cap=0.0, slopes=None, ws=None,
-             wsb=0, dt=0, st=None)
-    assert not set(kw) - set(a)
-    return list({**a, **kw}.values())
+    return _pack(dict(_BOTH, prefix_lens=A16, cu_q=A16, tree_mask=A16, mask_words=1, T=9, max_extend_len=8), kw)
+
+
+def test_argument_structure_matches_the_header(tmp_path):
+    """The packed bytes are the C structure: same size, every field where the compiler puts it."""
+    from mi355_attn import _lib
+    (tmp_path / "at.c").write_text('#include <stddef.h>\n#include <stdio.h>\n#include "mi355attn.h"\nint main(void) {\n' +
+                                   "".join(f'printf("%zu\\n", offsetof(M355ScoredArgs, {n}));\n' for n in _lib.SCORED_FIELDS) +
+                                   'printf("%zu\\n", sizeof(M355ScoredArgs)); return 0; }\n')
+    subprocess.run(["gcc", "-I", os.path.join(REPO, "include"), str(tmp_path / "at.c"), "-o", str(tmp_path / "at")], check=True)
+    where = [int(x) for x in subprocess.run([str(tmp_path / "at")], capture_output=True, text=True, check=True).stdout.split()]
+    assert where[-1] == _lib.SCORED_ARGS.size
+    n8, n4 = 21, 15
+    assert len(_lib.SCORED_FIELDS) == n8 + n4 and where[:-1] == [8 * i for i in range(n8)] + [8 * n8 + 4 * i for i in range(n4)]
 
 
 INVALID, UNSUPPORTED, WORKSPACE = -1, -2, -3
-COMMON = [(dict(q=None), INVALID), (dict(out=None), INVALID), (dict(k=A16 + 2), INVALID), (dict(qs=504), INVALID), (dict(os=516), INVALID),
-          (dict(pool=120), INVALID), (dict(pool=132), INVALID), (dict(S=0), INVALID), (dict(S=2 ** 31), INVALID), (dict(pts=7), INVALID),
-          (dict(cols=0), INVALID), (dict(B=-1), INVALID), (dict(T=-1), INVALID), (dict(Hq=9), INVALID), (dict(ps=0), INVALID),
-          (dict(D=96), UNSUPPORTED), (dict(dt=2), UNSUPPORTED), (dict(scale=0.0), INVALID), (dict(scale=float("nan")), INVALID),
-          (dict(cap=-1.0), INVALID), (dict(cap=float("inf")), INVALID), (dict(mx=0), INVALID)]
+COMMON = [(dict(q=None), INVALID), (dict(out=None), INVALID), (dict(k_pool=A16 + 2), INVALID), (dict(q_row_stride=504), INVALID),
+          (dict(o_row_stride=516), INVALID), (dict(pool_row_stride=120), INVALID), (dict(pool_row_stride=132), INVALID), (dict(pool_rows=0), INVALID),
+          (dict(pool_rows=2 ** 31), INVALID), (dict(pt_row_stride=7), INVALID), (dict(pt_cols=0), INVALID), (dict(B=-1), INVALID), (dict(T=-1), INVALID),
+          (dict(Hq=9), INVALID), (dict(page_size=0), INVALID), (dict(D=96), UNSUPPORTED), (dict(dtype=2), UNSUPPORTED), (dict(scale=0.0), INVALID),
+          (dict(scale=float("nan")), INVALID), (dict(softcap=-1.0), INVALID), (dict(softcap=float("inf")), INVALID), (dict(max_seq_len_hint=0), INVALID),
+          (dict(max_extend_len=0, prefix_lens=A16, cu_q=A16), INVALID)]
 
 
-@pytest.mark.parametrize("bad,code", COMMON + [(dict(win=-1), INVALID), (dict(lens=None), INVALID), (dict(pre=A16), INVALID),
-                                               (dict(cu=A16), INVALID), (dict(T=1), INVALID), (dict(pre=A16, cu=A16, ext=0), INVALID)])
+@pytest.mark.parametrize("bad,code", COMMON + [(dict(window=-1), INVALID), (dict(seq_lens=None), INVALID), (dict(prefix_lens=A16), INVALID),
+                                               (dict(cu_q=A16), INVALID), (dict(T=1), INVALID), (dict(tree_mask=A16), INVALID),
+                                               (dict(), WORKSPACE)])
 def test_scored_attn_refuses(bad, code):
     from mi355_attn import _lib
-    assert _lib.load().m355_scored_attn(*_scored_args(**bad)) == code
+    assert _lib.load().m355_scored_attn(_scored_args(**bad), None) == code
 
 
-@pytest.mark.parametrize("bad,code", COMMON + [(dict(pre=None), INVALID), (dict(cu=None), INVALID), (dict(mask=None), INVALID),
-                                               (dict(words=0), INVALID), (dict(nodes=33), INVALID), (dict(slopes=A16), INVALID)])
+@pytest.mark.parametrize("bad,code", COMMON + [(dict(prefix_lens=None), INVALID), (dict(cu_q=None), INVALID), (dict(tree_mask=None), INVALID),
+                                               (dict(mask_words=0), INVALID), (dict(max_extend_len=33), INVALID), (dict(slopes=A16), INVALID),
+                                               (dict(window=5), INVALID), (dict(seq_lens=A16), INVALID), (dict(doc_starts=A16), INVALID),
+                                               (dict(), WORKSPACE)])
 def test_tree_attn_refuses(bad, code):
     from mi355_attn import _lib
-    assert _lib.load().m355_tree_attn(*_tree_args(**bad)) == code
+    assert _lib.load().m355_tree_attn(_tree_args(**bad), None) == code
+
+
+def test_workspace_is_checked():
+    from mi355_attn import _lib
+    lib = _lib.load()
+    need = lib.m355_scored_workspace_bytes(2, 2, 8, 2, 64, 1, 100)
+    assert need > 0
+    for ws, n in ((A16, need - 1), (A16 + 16, need), (None, need)):
+        assert lib.m355_scored_attn(_scored_args(workspace=ws, workspace_bytes=n), None) == WORKSPACE
+    assert lib.m355_scored_attn(None, None) == INVALID and lib.m355_tree_attn(None, None) == INVALID
+    assert lib.m355_scored_workspace_bytes(0, 2, 8, 2, 64, 1, 100) == 0
 
 
 def test_empty_calls_do_nothing():
     from mi355_attn import _lib
     lib = _lib.load()
-    assert lib.m355_scored_attn(*_scored_args(T=0, q=None)) == 0 and lib.m355_tree_attn(*_tree_args(B=0, q=None)) == 0
+    assert lib.m355_scored_attn(_scored_args(T=0, q=None), None) == 0 and lib.m355_tree_attn(_tree_args(B=0, q=None), None) == 0
     assert lib.m355_tree_prepare(*([None] + [0] * 3 + [None] * 6 + [0, 0, 0, 0, None, 0, None, None, None])) == 0
     assert lib.m355_token_logprobs(None, 0, None, 0, 0, 10, 0, 1.0, None, None, None, None, None, 0, 0, None) == 0
 
