@@ -248,7 +248,7 @@ int m355_rope_kv_store(void *q, int64_t q_row_stride, void *k, int64_t k_row_str
 
 /* Attention over the paged KV pools with modified scores.  No counterpart in the reference, whose backends run a plain causal
  * softmax (torch_native_backend.py:25-193).  For query row t of request b at position pos, q head h, over its visible keys:
- *     x_k = scale * q[t,h] . K[k];   x_k = softcap * tanh(x_k / softcap)  (softcap > 0);
+ *     x_k = scale * q[t,h] . K[k];   x_k = softcap * tanh(x_k / softcap)  (softcap 2^-10 .. 1024; 0: not);
  *     x_k -= slopes[h] * |pos - k|   (slopes != NULL, fp32 [Hq]);
  *     out[t, h, :] = sum_k softmax(x)_k V[k, h / (Hq/Hkv), :]
  * m355_scored_attn: visible keys lo <= k < hi, lo = max(0, doc_starts[t], window > 0 ? pos - window + 1 : 0),
@@ -294,7 +294,7 @@ int m355_tree_attn(const M355ScoredArgs *args, void *stream);
  * tokens and brings cu_q[b+1] - cu_q[b] nodes (at most max_nodes <= M355_TREE_MAX_NODES); parents[cu_q[b] + j] is the index of
  * node j's parent inside the request, below j, or -1 for a node that follows the prefix directly (any other value is taken for
  * -1).  One launch:
- *     page_table[row_b, ceil(prefix/ps) + i] = new_pages[new_page_off[b] + i]        (new_pages NULL: the table is complete)
+ *     page_table[row_b, ceil(prefix/ps) + i] = new_pages[new_page_off[b] + i]        (new_pages int32 [new_page_count]; NULL, 0: the table is complete)
  *     positions[t] = prefix_lens[b] + depth of node t;    out_cache_loc[t] = slot of token prefix_lens[b] + j
  *     tree_mask[t, w] bit x = node 32 w + x is node t itself or one of its ancestors        (uint32 [T, mask_words])
  * Nodes take the request's next slots in node order, whatever their depth.  mask_words * 32 >= max_nodes.  A token past the
@@ -302,7 +302,7 @@ int m355_tree_attn(const M355ScoredArgs *args, void *stream);
 #define M355_TREE_MAX_NODES 1024
 int m355_tree_prepare(int32_t *page_table, int64_t pt_row_stride, int32_t pt_rows, int32_t pt_cols, const int64_t *page_table_ids,
                       const int64_t *prefix_lens, const int32_t *parents, const int32_t *cu_q, const int32_t *new_pages,
-                      const int32_t *new_page_off, int32_t B, int32_t T, int32_t max_nodes, int32_t page_size,
+                      const int32_t *new_page_off, int32_t new_page_count, int32_t B, int32_t T, int32_t max_nodes, int32_t page_size,
                       uint32_t *tree_mask, int32_t mask_words, int64_t *positions, int64_t *out_cache_loc, void *stream);
 
 /* Log probabilities of given tokens, entropy and top alternatives (the reference's sampler, layers/sampler.py:19-29, keeps

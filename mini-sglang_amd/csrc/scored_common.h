@@ -170,7 +170,7 @@ __device__ __forceinline__ uint32_t row_bits(const ScoredParams& p, const ReqSpa
 }
 
 // cap tanh(scale s / cap) log2(e) from the raw product s: tanh(x) = 1 - 2 / (1 + e^2x), exact at both ends (e^2x = 0 and inf);
-// near 0 its absolute error is a unit or two of cap 2^-24, which is what counts in an exponent.
+// near 0 its absolute error is a unit or two of cap 2^-24, which is what counts in an exponent (hence no caps beyond 1024).
 __device__ __forceinline__ float cap_score(const ScoredParams& p, float s) {
     return fmaf(-2.f * p.cap_log2, __builtin_amdgcn_rcpf(1.f + exp2_fast(s * p.cap_rate)), p.cap_log2);
 }

@@ -15,7 +15,7 @@ __global__ __launch_bounds__(256) void tree_prepare_kernel(int32_t* __restrict__
                                                            const int64_t* __restrict__ page_table_ids, const int64_t* __restrict__ prefix_lens,
                                                            const int32_t* __restrict__ parents, const int32_t* __restrict__ cu_q,
                                                            const int32_t* __restrict__ new_pages, const int32_t* __restrict__ new_page_off,
-                                                           int32_t T, int32_t ps, uint32_t* __restrict__ mask, int32_t words,
+                                                           int32_t new_page_count, int32_t T, int32_t ps, uint32_t* __restrict__ mask, int32_t words,
                                                            int64_t* __restrict__ positions, int64_t* __restrict__ out_cache_loc) {
     __shared__ int32_t par[kMaxNodes];
     const int b = blockIdx.x;
@@ -27,8 +27,9 @@ __global__ __launch_bounds__(256) void tree_prepare_kernel(int32_t* __restrict__
     const bool row_ok = row >= 0 && row < pt_rows;
     int32_t* const pt = page_table + (row_ok ? row : 0) * pt_stride;
     const int32_t first = (int32_t)(((int64_t)P + ps - 1) / ps);        // the first column the prefix does not use
-    const int32_t* const fresh = new_pages ? new_pages + new_page_off[b] : nullptr;
-    const int n_fresh = new_pages ? imax(new_page_off[b + 1] - new_page_off[b], 0) : 0;
+    const int32_t off = new_pages ? imin(imax(new_page_off[b], 0), new_page_count) : 0;
+    const int32_t* const fresh = new_pages + off;
+    const int n_fresh = new_pages ? imin(imax(new_page_off[b + 1] - off, 0), new_page_count - off) : 0;
     if (row_ok)
         for (int i = threadIdx.x; i < n_fresh && first + i < pt_cols; i += 256) pt[first + i] = fresh[i];
     __syncthreads();
@@ -64,16 +65,16 @@ using namespace m355;
 
 extern "C" int m355_tree_prepare(int32_t* page_table, int64_t pt_row_stride, int32_t pt_rows, int32_t pt_cols, const int64_t* page_table_ids,
                                  const int64_t* prefix_lens, const int32_t* parents, const int32_t* cu_q, const int32_t* new_pages,
-                                 const int32_t* new_page_off, int32_t B, int32_t T, int32_t max_nodes, int32_t page_size,
+                                 const int32_t* new_page_off, int32_t new_page_count, int32_t B, int32_t T, int32_t max_nodes, int32_t page_size,
                                  uint32_t* tree_mask, int32_t mask_words, int64_t* positions, int64_t* out_cache_loc, void* stream) {
     if (T == 0 || B == 0) return M355_OK;
     if (!page_table || !page_table_ids || !prefix_lens || !parents || !cu_q || !tree_mask || !positions || !out_cache_loc) return M355_ERR_INVALID_ARG;
     if (B < 0 || T < 0 || page_size <= 0 || pt_rows <= 0 || pt_cols <= 0 || pt_row_stride < pt_cols || max_nodes <= 0) return M355_ERR_INVALID_ARG;
-    if ((new_pages == nullptr) != (new_page_off == nullptr)) return M355_ERR_INVALID_ARG;
+    if ((new_pages == nullptr) != (new_page_off == nullptr) || new_page_count < 0) return M355_ERR_INVALID_ARG;
     if (mask_words <= 0 || (int64_t)mask_words * 32 < max_nodes) return M355_ERR_INVALID_ARG;
     if (max_nodes > kMaxNodes || mask_words > kMaxNodes / 32) return M355_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(tree_prepare_kernel, dim3((unsigned)B), dim3(256), 0, (hipStream_t)stream, page_table, pt_row_stride, pt_rows, pt_cols,
-                       page_table_ids, prefix_lens, parents, cu_q, new_pages, new_page_off, T, page_size, tree_mask, mask_words, positions,
+                       page_table_ids, prefix_lens, parents, cu_q, new_pages, new_page_off, new_page_count, T, page_size, tree_mask, mask_words, positions,
                        out_cache_loc);
     return check_launch();
 }

@@ -96,7 +96,7 @@ SIGNATURES = {
     "m355_scored_attn": (c_int32, [c_char_p, c_void_p]),        # M355ScoredArgs, packed (SCORED_ARGS)
     "m355_tree_attn": (c_int32, [c_char_p, c_void_p]),
     "m355_tree_prepare": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                    c_int32, c_int32, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
+                                    c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
     "m355_token_logprobs_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32]),
     "m355_token_logprobs": (c_int32, [c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p,
                                       c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p]),

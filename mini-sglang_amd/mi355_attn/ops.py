@@ -551,7 +551,7 @@ def tree_prepare(page_table: torch.Tensor, page_table_ids: torch.Tensor, prefix_
     pt_rows, pt_cols, pt_stride = _table("tree_prepare", page_table, page_size)
     ids, pre = _vector("page_table_ids", page_table_ids, torch.int64, B), _vector("prefix_lens", prefix_lens, torch.int64, B)
     par, cu = _vector("parents", parents, torch.int32, T), _vector("cu_q", cu_q, torch.int32, B + 1)
-    fresh = off = None
+    fresh, off, n = None, None, 0
     if (new_pages is None) != (new_page_off is None):
         raise _lib.MI355AttnError("tree_prepare: new_pages and new_page_off go together")
     if new_pages is not None:
@@ -564,7 +564,7 @@ def tree_prepare(page_table: torch.Tensor, page_table_ids: torch.Tensor, prefix_
     words = (max_nodes + 31) // 32
     mask = parents.new_empty((T, words))
     positions, slots = prefix_lens.new_empty((2, T)).unbind()
-    code = _lib.load().m355_tree_prepare(page_table.data_ptr(), pt_stride, pt_rows, pt_cols, ids, pre, par, cu, fresh, off, B, T, max_nodes,
+    code = _lib.load().m355_tree_prepare(page_table.data_ptr(), pt_stride, pt_rows, pt_cols, ids, pre, par, cu, fresh, off, n, B, T, max_nodes,
                                          page_size, mask.data_ptr(), words, positions.data_ptr(), slots.data_ptr(), current_stream())
     if code:
         check(code, "m355_tree_prepare")

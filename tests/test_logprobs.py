@@ -91,6 +91,15 @@ def test_masked_vocabularies_and_rows_without_a_distribution():
         check(x, torch.tensor([[0, 5], [6000, 1], [3, 8], [0, 9000], [0, 77], [0, 1], [3, 4], [-1, 9001]]), 6)
 
 
+def test_rows_of_nan():
+    x = torch.randn((4, 20001), generator=torch.Generator().manual_seed(9))
+    x[0, :] = float("nan")
+    x[1, ::2] = float("nan")
+    x[2, -3:] = float("nan")
+    x[3, 100] = -float("nan")
+    check(x, torch.tensor([0, 1, 2, 3]), 40)
+
+
 def test_tokens_outside_the_vocabulary():
     x = torch.randn((3, 100), generator=torch.Generator().manual_seed(2))
     check(x, torch.tensor([-1, 100, 2 ** 40]), 0)

@@ -280,6 +280,44 @@ def test_captured_graph_replays():
         assert torch.equal(out, eager)
 
 
+@pytest.mark.parametrize("B,Hkv", [(130, 1), (70, 2), (300, 1)])
+def test_more_requests_than_lanes(B, Hkv):
+    """Batches of more requests than a wave has lanes, lengths from 1 to a few hundred, some requests without rows."""
+    lens = [1 + (i * 37) % 311 for i in range(B)]
+    c = Case(21, BF, (4 * Hkv, Hkv, 64), 16, [n - 1 for n in lens], [1] * B)
+    check(c.run(decode=True, softcap=30.0), *c.want(softcap=30.0))
+    ext = [0 if i % 9 == 0 else 1 + i % 6 for i in range(B)]
+    c = Case(22, BF, (4 * Hkv, Hkv, 64), 16, [n - 1 for n in lens], ext)
+    check(c.run(window=100), *c.want(window=100))
+
+
+def test_hints_that_promise_too_little():
+    """More rows per request than max_extend_len said: rows past it may be left out, nothing else suffers."""
+    from mi355_attn import ops
+    c = Case(23, BF, (4, 1, 64), 16, [40, 3], [30, 2])
+    args = (c.q.reshape(c.T, -1).to(DEV), c.pool(c.k), c.pool(c.v), c.table.to(DEV), c.rows.to(DEV), torch.tensor(c.len, device=DEV), 16, 4)
+    form = dict(prefix_lens=torch.tensor(c.pre, device=DEV), cu_q=torch.tensor(c.cu, dtype=torch.int32, device=DEV))
+    want, tol = c.want()
+    for ext, mx in ((2, 1), (4, 200), (30, 1)):
+        got = ops.scored_attn(*args, mx, max_extend_len=ext, **form).double().cpu().view(want.shape)
+        rows = [*range(min(ext, 30)), 30, 31]
+        assert bool(((got - want).abs() <= tol)[rows].all()), (ext, mx)
+
+
+def test_lengths_that_contradict_the_rows():
+    """cu_q that runs backwards or past q, lengths past the table: in-bounds work, finite pools give finite rows or none."""
+    from mi355_attn import ops
+    c = Case(24, BF, (4, 2, 64), 16, [30, 5], [4, 4])
+    c.k.nan_to_num_(), c.v.nan_to_num_()
+    table = c.table.clamp(max=3)
+    for cu, pre, lens in (([0, 4, 100], [30, 5], [34, 9]), ([4, 0, 8], [30, 5], [34, 9]), ([0, 4, 8], [-7, 2 ** 40], [2 ** 40, -3]), ([0, 0, 0], [1, 1], [1, 1])):
+        out = torch.zeros((8, 256), dtype=BF, device=DEV)
+        ops.scored_attn(c.q.reshape(8, -1).to(DEV), c.pool(c.k).nan_to_num(), c.pool(c.v).nan_to_num(), table.to(DEV), c.rows.to(DEV),
+                        torch.tensor(lens, device=DEV), 16, 4, 40, prefix_lens=torch.tensor(pre, device=DEV),
+                        cu_q=torch.tensor(cu, dtype=torch.int32, device=DEV), max_extend_len=8, out=out)
+        torch.cuda.synchronize()
+
+
 def test_refusals():
     from mi355_attn import MI355AttnBackend  # noqa: F401  (the package imports)
     from mi355_attn._lib import MI355AttnError

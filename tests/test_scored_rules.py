@@ -128,7 +128,8 @@ COMMON = [(dict(q=None), INVALID), (dict(out=None), INVALID), (dict(k_pool=A16 +
           (dict(o_row_stride=516), INVALID), (dict(pool_row_stride=120), INVALID), (dict(pool_row_stride=132), INVALID), (dict(pool_rows=0), INVALID),
           (dict(pool_rows=2 ** 31), INVALID), (dict(pt_row_stride=7), INVALID), (dict(pt_cols=0), INVALID), (dict(B=-1), INVALID), (dict(T=-1), INVALID),
           (dict(Hq=9), INVALID), (dict(page_size=0), INVALID), (dict(D=96), UNSUPPORTED), (dict(dtype=2), UNSUPPORTED), (dict(scale=0.0), INVALID),
-          (dict(scale=float("nan")), INVALID), (dict(softcap=-1.0), INVALID), (dict(softcap=float("inf")), INVALID), (dict(max_seq_len_hint=0), INVALID),
+          (dict(scale=float("nan")), INVALID), (dict(softcap=-1.0), INVALID), (dict(softcap=float("inf")), INVALID), (dict(softcap=1e-4), INVALID), (dict(softcap=2000.0), INVALID),
+          (dict(softcap=float("nan")), INVALID), (dict(scale=1e20), INVALID), (dict(max_seq_len_hint=0), INVALID),
           (dict(max_extend_len=0, prefix_lens=A16, cu_q=A16), INVALID)]
 
 
@@ -164,15 +165,15 @@ def test_empty_calls_do_nothing():
     from mi355_attn import _lib
     lib = _lib.load()
     assert lib.m355_scored_attn(_scored_args(T=0, q=None), None) == 0 and lib.m355_tree_attn(_tree_args(B=0, q=None), None) == 0
-    assert lib.m355_tree_prepare(*([None] + [0] * 3 + [None] * 6 + [0, 0, 0, 0, None, 0, None, None, None])) == 0
+    assert lib.m355_tree_prepare(*([None] + [0] * 3 + [None] * 6 + [0, 0, 0, 0, 0, None, 0, None, None, None])) == 0
     assert lib.m355_token_logprobs(None, 0, None, 0, 0, 10, 0, 1.0, None, None, None, None, None, 0, 0, None) == 0
 
 
 def test_tree_prepare_refuses():
     from mi355_attn import _lib
-    base = dict(pt=A16, pts=8, rows=4, cols=8, ids=A16, pre=A16, par=A16, cu=A16, pages=A16, off=A16, B=2, T=9, nodes=8, ps=16,
+    base = dict(pt=A16, pts=8, rows=4, cols=8, ids=A16, pre=A16, par=A16, cu=A16, pages=A16, off=A16, count=4, B=2, T=9, nodes=8, ps=16,
                 mask=A16, words=1, pos=A16, loc=A16, st=None)
-    for bad, code in ((dict(par=None), INVALID), (dict(off=None), INVALID), (dict(pts=4), INVALID), (dict(nodes=0), INVALID),
+    for bad, code in ((dict(par=None), INVALID), (dict(off=None), INVALID), (dict(count=-1), INVALID), (dict(pts=4), INVALID), (dict(nodes=0), INVALID),
                       (dict(nodes=33), INVALID), (dict(ps=0), INVALID), (dict(nodes=1025, words=33), UNSUPPORTED), (dict(words=33), UNSUPPORTED)):
         assert _lib.load().m355_tree_prepare(*{**base, **bad}.values()) == code, bad
 

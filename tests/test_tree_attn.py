@@ -89,6 +89,16 @@ def test_tree_metadata_past_the_table():
     assert bool((table == 5).all())
 
 
+def test_page_offsets_past_the_list_read_nothing():
+    """Offsets that contradict the list of new pages: no read leaves it, other requests are as they were."""
+    from mi355_attn import ops
+    table = torch.full((3, 8), 5, dtype=torch.int32, device=DEV)
+    ops.tree_prepare(table, torch.tensor([0, 1], device=DEV), torch.tensor([8, 8], device=DEV), torch.tensor([-1, 0, -1, 0], dtype=torch.int32, device=DEV),
+                     torch.tensor([0, 2, 4], dtype=torch.int32, device=DEV), 4, 2, new_pages=torch.tensor([9, 10], dtype=torch.int32, device=DEV),
+                     new_page_off=torch.tensor([0, 1, 2 ** 30], dtype=torch.int32, device=DEV))
+    assert table[:, 2].tolist() == [9, 10, 5] and bool((table[:, 3:] == 5).all())
+
+
 def test_long_chain_and_largest_tree():
     n = 1024
     c = Case(3, BF, (1, 1, 64), 16, [5], [n])
