@@ -670,37 +670,41 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
         }
 }
 
-// out[row, head, :] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the parts of a row, RB part rows apart: D/4 lanes per
-// (row, head), four floats each, eight parts' loads in flight per lane.
-template <int D, int RB, bool F16>
+// out[row, head, :] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the parts of a row, RB part rows apart.  D/4 lanes hold a
+// row, four floats each; GROUPS of them take every GROUPS-th part with eight parts' loads in flight per lane, and meet in LDS.
+// One group where there are rows enough to fill the chip, eight where there are not and the launch is a chain of latencies (128
+// rows of 32 parts: 5.9 us with one).
+template <int D, int RB, int GROUPS, bool F16>
 __global__ __launch_bounds__(256) void scored_merge_kernel(const ScoredParams p) {
-    constexpr int LPI = D / 4, CH = 8;
-    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPI;
-    const int li = threadIdx.x % LPI;
+    constexpr int LPI = D / 4, CH = 8, PER = 256 / (LPI * GROUPS);  // rows of a workgroup
+    __shared__ f32x4 jo[GROUPS > 1 ? 256 : 1];
+    __shared__ float2 jm[GROUPS > 1 ? PER * GROUPS : 1];
+    const int li = threadIdx.x % LPI, gr = threadIdx.x / LPI % GROUPS, slot = threadIdx.x / (LPI * GROUPS);
+    const int64_t item = (int64_t)blockIdx.x * PER + slot;
     const int64_t row = item / p.Hq, head = item - row * p.Hq;
     const int64_t r0 = p.cu_q ? imax(p.cu_q[0], 0) : 0, r1 = p.cu_q ? imin(p.cu_q[p.B], p.T) : imin(p.B, p.T);
-    if (row < r0 || row >= r1) return;                              // rows of no request: left as they were
-    const int2 of = p.part_of[item];
-    const int n = of.y;
+    const bool mine = row >= r0 && row < r1;                        // (rows of no request: left as they were)
+    const int2 of = mine ? p.part_of[item] : make_int2(0, 0);
     // 1: written by the attention kernel.  (A row that no share reached - lengths that contradict cu_q - has no entry: nothing out of
     // the parts is read for it.)
-    if (n <= 1 || of.x < 0 || of.x / RB + (int64_t)n > p.max_parts) return;
+    const int n = of.x < 0 || of.y <= 1 || of.x / RB + (int64_t)of.y > p.max_parts ? 0 : of.y;
+    if (GROUPS == 1 && n == 0) return;
     const float* base = p.part + (int64_t)of.x * (D + 4);
     float mx = -INFINITY, den = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < n; s0 += CH) {
+    for (int s0 = gr; s0 < n; s0 += CH * GROUPS) {
         float2 ml[CH];
         f32x4 o[CH];
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
-            const float* ps = base + (int64_t)imin(s0 + k, n - 1) * (RB * (D + 4));
+            const float* ps = base + (int64_t)imin(s0 + k * GROUPS, n - 1) * (RB * (D + 4));
             ml[k] = *reinterpret_cast<const float2*>(ps + D);
             o[k] = *reinterpret_cast<const f32x4*>(ps + 4 * li);
         }
         float mn = mx;
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
-            if (s0 + k >= n) { ml[k] = make_float2(-INFINITY, 0.f); o[k] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+            if (s0 + k * GROUPS >= n) { ml[k] = make_float2(-INFINITY, 0.f); o[k] = f32x4{0.f, 0.f, 0.f, 0.f}; }
             mn = fmaxf(mn, ml[k].x);
         }
         const float mu = finite_max(mn), rs = exp2_fast(mx - mu);
@@ -713,6 +717,24 @@ __global__ __launch_bounds__(256) void scored_merge_kernel(const ScoredParams p)
             acc += o[k] * w;
         }
         mx = mn;
+    }
+    if constexpr (GROUPS > 1) {
+        jo[threadIdx.x] = acc;
+        if (li == 0) jm[slot * GROUPS + gr] = make_float2(mx, den);
+        __syncthreads();
+        if (gr || n == 0) return;
+        float mn = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) mn = fmaxf(mn, jm[slot * GROUPS + g].x);
+        const float mu = finite_max(mn);
+        den = 0.f;
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            const float w = exp2_fast(jm[slot * GROUPS + g].x - mu);
+            den = fmaf(w, jm[slot * GROUPS + g].y, den);
+            acc += jo[(slot * GROUPS + g) * LPI + li] * w;
+        }
     }
     const float inv = 1.f / den;
     uint2 w = {0u, 0u};
@@ -781,6 +803,13 @@ static int check_args(const M355ScoredArgs& a) {
     return M355_OK;
 }
 
+template <int D, int RB, bool F16>
+static void launch_merge(const ScoredParams& p, int64_t rows, hipStream_t st) {
+    constexpr int LPI = D / 4;
+    if (rows * LPI < 256 * 256) hipLaunchKernelGGL((scored_merge_kernel<D, RB, 8, F16>), dim3((unsigned)((rows * LPI * 8 + 255) / 256)), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((scored_merge_kernel<D, RB, 1, F16>), dim3((unsigned)((rows * LPI + 255) / 256)), dim3(256), 0, st, p);
+}
+
 template <int D, bool MOD, bool F16>
 static void launch_kernels(const ScoredParams& p, const ScoredCut& c, hipStream_t st) {
     if (c.wide) {
@@ -790,9 +819,9 @@ static void launch_kernels(const ScoredParams& p, const ScoredCut& c, hipStream_
         hipLaunchKernelGGL((scored_few_kernel<D, MOD, F16>), dim3((unsigned)c.grid), dim3(64 * kFewWaves), 0, st, p);
     }
     if (p.slots) {
-        const dim3 grid((unsigned)(((int64_t)p.T * p.Hq * (D / 4) + 255) / 256));
-        if (c.wide) hipLaunchKernelGGL((scored_merge_kernel<D, kWideRows, F16>), grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((scored_merge_kernel<D, kFewRows, F16>), grid, dim3(256), 0, st, p);
+        const int64_t rows = (int64_t)p.T * p.Hq;
+        if (c.wide) launch_merge<D, kWideRows, F16>(p, rows, st);
+        else launch_merge<D, kFewRows, F16>(p, rows, st);
     }
 }
 
