@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(const Logpr
     __shared__ uint64_t floor_key;
     const int tid = threadIdx.x;
     const int64_t t = blockIdx.x;
-    const int sp = blockIdx.y, k = p.k;
+    const int sp = blockIdx.y, k = p.k, k2 = (k + 1) & ~1;          // the list's candidates start at an even place
     // rows of any alignment: loads start at the 16 bytes that hold the row's first logit, and what lies outside the row in the
     // first and last of them is taken for -inf (those 16 bytes hold a logit of the row: they are mapped)
     const uintptr_t addr = (uintptr_t)(p.logits + t * p.row_bytes);
@@ -241,12 +241,12 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(const Logpr
                     const uint64_t key = logit_key(logit_at<DT>(row16, (int64_t)i + skip), (uint32_t)i);
                     if (key > mine) mine = key;
                 }
-                list[kMaxTop + tid] = mine;
+                list[k2 + tid] = mine;
                 if (tid == 0) floor_key = 0;
                 __syncthreads();
                 int above = 0;
 #pragma unroll 4
-                for (int u = 0; u < kThreads; ++u) above += list[kMaxTop + u] > mine ? 1 : 0;
+                for (int u = 0; u < kThreads; ++u) above += list[k2 + u] > mine ? 1 : 0;
                 if (mine && above == k - 1) floor_key = mine;
                 __syncthreads();
                 if (floor_key > at_least) at_least = floor_key;
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(const Logpr
                         const uint64_t key = logit_key(x, (uint32_t)i);
                         if (i >= 0 && i < p.V && key >= at_least) {
                             const int at = atomicAdd(&count, 1);
-                            if (at < kCand) list[kMaxTop + at] = key;
+                            if (at < kCand) list[k2 + at] = key;
                         }
                     }
                 }
@@ -271,11 +271,11 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(const Logpr
             const int found = count;
             if (found <= kCand) {
                 if (tid < kMaxTop) ranked[tid] = 0;
-                if (tid < 2) list[kMaxTop + found + tid] = 0;
+                if (tid < 2) list[k2 + found + tid] = 0;
                 __syncthreads();
-                rank_keys<kThreads>(list, kMaxTop + found, k, ranked, tid);
+                rank_keys<kThreads>(list, k2 + found, k, ranked, tid);
                 __syncthreads();
-                if (tid < kMaxTop) list[tid] = ranked[tid];
+                if (tid < k) list[tid] = ranked[tid];
                 least = ranked[k - 1];
                 if (tid == 0) count = 0;
                 break;
