@@ -386,7 +386,10 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
     }
-    const float slope = MOD && p.slopes ? p.slopes[h * p.G + g] * kLog2e : 0.f;
+    // a score in log2 units is unit * s, s being what `modify` leaves: a capped one is kept as -1 / (1 + e^2x), which is its tanh but for
+    // a factor and a constant; the constant drops out of the softmax and the factor into the exponent's multiply-add
+    const float unit = !MOD ? p.scale_log2 : p.cap_log2 > 0.f ? 2.f * p.cap_log2 : 1.f;
+    const float slope = MOD && p.slopes ? p.slopes[h * p.G + g] * kLog2e / unit : 0.f;
     int lo_wg, hi_wg;
     if (p.doc_starts) {
         __syncthreads();
@@ -470,7 +473,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     auto modify = [&](f32x16& s, const int base) {
         if (p.cap_log2 > 0.f) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = cap_score(p, s[i]);
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_rcpf(-1.f - exp2_fast(s[i] * p.cap_rate));
         } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] *= p.scale_log2;
@@ -500,8 +503,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     auto new_max = [&](float mx) {
         float a, e;
         lane_pair<32>(mx, a, e);
-        mx = fmaxf(a, e);
-        if constexpr (!MOD) mx *= p.scale_log2;
+        mx = fmaxf(a, e) * unit;
         const float m_new = mx > m_run + kLazy ? mx : m_run;
         const float alpha = m_new == m_run ? 1.f : exp2_fast(m_run - m_new);
         m_run = m_new;
@@ -517,7 +519,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
         const float mu = finite_max(m_run);
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { s[i] = exp2_fast(MOD ? s[i] - mu : fmaf(s[i], p.scale_log2, -mu)); sum += s[i]; }
+        for (int i = 0; i < 16; ++i) { s[i] = exp2_fast(fmaf(s[i], unit, -mu)); sum += s[i]; }
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             u32x4 w;
