@@ -55,7 +55,7 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 //   S^T[key, row]  = K[32 x D] . Q^T[D x 16]   v_mfma_f32_16x16x32: a lane owns one row and 8 of the tile's keys
 //   O^T[d, row]   += V^T[D x 32] . P^T[32 x 16]   P^T is the S^T accumulator rounded in place, V^T is read transposed
 // Bound by HBM.  Two waves: the LDS then holds two workgroups a CU at head_dim 128 and four at 64, whose starts and ends overlap
-// (16 requests of 20 000 to 32 768 tokens, 222 MB: 41.6 us, 5.3 TB/s; with four waves 49.8, with one 58.7).  More rows go to
+// (16 requests of 20 000 to 32 768 tokens, 222 MB: 40.6 us, 5.5 TB/s; with four waves 49.8, with one 58.7).  More rows go to
 // the other kernel: with 32 rows here, 16 requests of 2 250 tokens took 45 us against 29.
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 16, kFewWaves = 2, kWideRows = 128;
@@ -303,6 +303,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
 // pair of 32-key tiles at a time, brought into LDS once per workgroup by LDS-DMA (two pairs deep).  The matrix products are
 // those of prefill_attn.hip (v_mfma_f32_32x32x16, a lane owns one row and 16 of a tile's keys); what differs is the score
 // stage between them and the range that is walked.
+//
+// Bound by vector issue: per score a multiply-add, an exponential, a sum, half a maximum and a quarter of a conversion stand beside
+// 4 D matrix flops; a cap puts two more transcendentals and two plain instructions on top.  A prompt of 8192 tokens (32 / 8 heads of
+// 128): 590 us plain, 930 TFLOP/s, 700 capped (capping one tile beside the other's matrix product in source order, forced or
+// not: within 1%; the SIMD's other wave already fills the gaps).  16 capped turns of 384 to 640 tokens over 1024 cached: 275
+// us, 635 TFLOP/s, in four rounds of workgroups the last of which is partly empty.  Documents of ~700 tokens at head_dim 64: 128 us, 470
+// TFLOP/s, half the matrix work per score and 17 key pairs a block, of which the first and last are masked.  Eight waves a workgroup
+// or 64 rows a wave spill or leave the chip emptier: no gain.
 // ------------------------------------------------------------------------------------------------------------------------
 template <int D, bool MOD, bool F16, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams p) {
@@ -675,7 +683,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
 // out[row, head, :] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the parts of a row, RB part rows apart.  D/4 lanes hold a
 // row, four floats each; GROUPS of them take every GROUPS-th part with eight parts' loads in flight per lane, and meet in LDS.
 // One group where there are rows enough to fill the chip, eight where there are not and the launch is a chain of latencies (128
-// rows of 32 parts: 5.9 us with one).
+// rows of 32 parts: 4.7 us against 5.9 with one; 4096 rows: 4.3 with one, 9.3 with eight).
 template <int D, int RB, int GROUPS, bool F16>
 __global__ __launch_bounds__(256) void scored_merge_kernel(const ScoredParams p) {
     constexpr int LPI = D / 4, CH = 8, PER = 256 / (LPI * GROUPS);  // rows of a workgroup

@@ -1,7 +1,8 @@
 // Metadata of a batch of draft trees in one launch: the new pages enter the page table, every node gets its position
 // (prefix + depth), its KV slot (the request's next slots in node order) and the mask of its ancestors.
 //
-// Whole numbers only; a few hundred nodes, so launch latency bounds it.  One workgroup per request holds the parents in LDS;
+// Whole numbers only; a few hundred nodes, so launch latency bounds it (1 tree of 8 nodes 2.8 us, 16 trees of 17 to 48 4.3, 4 of 64
+// 4.8: three dependent trips to memory, then the climb in LDS).  One workgroup per request holds the parents in LDS;
 // one thread per (node, mask word) climbs from the node towards the root - a parent is accepted only below its child, so
 // every climb ends - and sets the bits that fall into its word.  No thread waits for another node's mask, which a
 // row = parent's row | own bit recurrence would.
