@@ -127,6 +127,7 @@ class GraphedDecode:
         self.pos, self.loc = torch.empty_like(self.seq_lens), torch.empty_like(self.seq_lens)
         self.out = torch.zeros((B, max(n_steps, 1)), dtype=torch.int64, device=dev)
         self.step = torch.zeros((1, 1), dtype=torch.int64, device=dev)
+        batch._no_open_tree()
         batch.mode = m.Mode.DECODE
         batch.input_ids, batch.output_ids = self.ids, None
         batch.seq_lens, batch.positions, batch.out_cache_loc = self.seq_lens, self.pos, self.loc
@@ -285,6 +286,8 @@ def correctness_test(runner, bench_args: BenchArgs, rank_print):
 
 
 def latency_test(runner, bench_args: BenchArgs, bs: int, il: int, ol: int, rank_print, tp_size: int):
+    if sum(map(bool, (bench_args.graph, bench_args.speculate, bench_args.top_logprobs))) > 1:
+        raise ValueError("latency mode takes one of --graph, --speculate and --top-logprobs")
     shape = runner.model.shape
     sync = torch.cuda.synchronize
     result = None

@@ -80,6 +80,12 @@ def _any(options: dict) -> bool:
     return any(v is not None and (isinstance(v, torch.Tensor) or bool(v)) for v in options.values())
 
 
+def _modified(layer, batch) -> bool:
+    """A layer or batch for the scored kernels.  Asked in every layer of every step, so without building the two dicts."""
+    return bool(getattr(layer, "logit_cap", 0.0) or getattr(layer, "window", 0) or getattr(layer, "slopes", None) is not None
+                or getattr(batch, "doc_starts", None) is not None or getattr(batch, "bidir_lens", None) is not None)
+
+
 class MI355AttnBackend:
     def __init__(self, model_runner):
         self.device = model_runner.device
@@ -173,9 +179,8 @@ class MI355AttnBackend:
             md.first_layer = layer.layer_id
         k_pool, v_pool = batch.kvcache.get_kv_cache(layer.layer_id)
         B = q.shape[0]
-        mods, masks = _modifiers(layer), _masks(batch)
-        if _any(mods) or _any(masks):
-            return self._scored(q, k, v, layer, batch, mods, masks, {})
+        if _modified(layer, batch):
+            return self._scored(q, k, v, layer, batch, {})
         fuse = (self.fused_store and k is not None and k.dtype == k_pool.dtype
                 and v.dtype == v_pool.dtype and k.stride(-1) == 1 and v.stride(-1) == 1)
         if not fuse:
@@ -201,7 +206,7 @@ class MI355AttnBackend:
                                     k_new=k if fuse else None, v_new=v if fuse else None)
         return o if Gp == G else _drop_pad(o, Hkv, G, Gp, D)
 
-    def _scored(self, q, k, v, layer, batch, mods, masks, form):
+    def _scored(self, q, k, v, layer, batch, form):
         """Decode or extend attention with modified scores; `form` holds the ragged form's arguments."""
         self._store_kv(k, v, layer, batch)
         k_pool, v_pool = batch.kvcache.get_kv_cache(layer.layer_id)
@@ -209,7 +214,8 @@ class MI355AttnBackend:
         need = ops.scored_workspace_bytes(batch.seq_lens.numel(), q.shape[0], layer.num_heads, layer.num_kv_heads, layer.head_dim,
                                           form.get("max_extend_len", 1), md.max_seq_len)
         return ops.scored_attn(q, k_pool, v_pool, batch.page_manager.page_table, batch.page_table_ids, batch.seq_lens, self.page_size,
-                               layer.num_heads, md.max_seq_len, workspace=self._ws(need, q.device), **form, **mods, **masks)
+                               layer.num_heads, md.max_seq_len, workspace=self._ws(need, q.device), **form,
+                               **_modifiers(layer), **_masks(batch))
 
     def forward_tree(self, q, k, v, layer, batch):
         """Attention of a batch of draft trees (Batch.prepare_for_tree): every node over its request's cached tokens and its
@@ -222,6 +228,8 @@ class MI355AttnBackend:
         mods = _modifiers(layer)
         if mods.pop("window"):
             raise ops._lib.MI355AttnError("MI355AttnBackend: draft trees are not supported in layers with a window")
+        if _any(_masks(batch)):
+            raise ops._lib.MI355AttnError("MI355AttnBackend: draft trees take no document or prefix mask")
         self._store_kv(k, v, layer, batch)
         k_pool, v_pool = batch.kvcache.get_kv_cache(layer.layer_id)
         need = ops.scored_workspace_bytes(batch.seq_lens.numel(), q.shape[0], layer.num_heads, layer.num_kv_heads, layer.head_dim,
@@ -231,13 +239,12 @@ class MI355AttnBackend:
 
     def forward_extend(self, q, k, v, layer, batch):
         md = self.forward_metadata
-        if md is None or md.decode or self._new_forward(md, layer):
+        if md is None or md.decode or md.tree or self._new_forward(md, layer):
             self.init_forward_metadata(batch)
             md = self.forward_metadata
             md.first_layer = layer.layer_id
-        mods, masks = _modifiers(layer), _masks(batch)
-        if _any(mods) or _any(masks):
-            return self._scored(q, k, v, layer, batch, mods, masks,
+        if _modified(layer, batch):
+            return self._scored(q, k, v, layer, batch,
                                 {"prefix_lens": batch.prefix_lens, "cu_q": md.cu_q, "max_extend_len": md.max_extend_len})
         self._store_kv(k, v, layer, batch)       # first: the new tokens' K/V are read back from the pool
         k_pool, v_pool = batch.kvcache.get_kv_cache(layer.layer_id)

@@ -340,6 +340,7 @@ class Batch:
         self.seq_lens_host = lens
         self.seq_lens = _h2d(np.asarray(lens, dtype=np.int64), self.device)
         self.tree = self.tree_lens_host = self.cu_q = self.positions = self.out_cache_loc = self.input_ids = None
+        self.doc_starts = self.bidir_lens = None
         self._tree_parents, self._tree_pages, self.mode = [], [], Mode.DECODE
 
     # ---- bookkeeping kept working (engine/batch.py:345-464)

@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import functools
 import math
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -478,6 +479,16 @@ def scored_workspace_bytes(B: int, T: int, Hq: int, Hkv: int, D: int, max_extend
     return int(_lib.load().m355_scored_workspace_bytes(B, T, Hq, Hkv, D, max_extend_len, max_seq_len))
 
 
+def _scored_call(entry: str, *fields) -> None:
+    try:
+        args = _lib.SCORED_ARGS.pack(*fields)
+    except struct.error as e:
+        raise _lib.MI355AttnError(f"{entry}: an argument does not fit its field: {e}") from None
+    code = getattr(_lib.load(), entry)(args, current_stream())
+    if code:
+        check(code, entry)
+
+
 def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
                 page_table_ids: torch.Tensor, seq_lens: torch.Tensor, page_size: int, num_heads: int, max_seq_len: int, *,
                 prefix_lens: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None, max_extend_len: int = 1,
@@ -517,13 +528,10 @@ def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, pag
     out, o_stride = _out_rows("scored_attn", q2, out, T, W)
     need = 0 if workspace is not None else scored_workspace_bytes(B, T, num_heads, Hkv, D, max_extend_len, max_seq_len)
     held, ws_ptr, ws_bytes = _scratch(workspace, need, q.device)
-    code = _lib.load().m355_scored_attn(
-        _lib.SCORED_ARGS.pack(q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ids, lens, pre, cu, out.data_ptr(),
-                              slope_ptr, doc_ptr, bidir_ptr, 0, 0, ws_ptr, q2.stride(0) if T > 1 else W, o_stride, pitch, S, pt_stride, ws_bytes,
-                              pt_rows, pt_cols, B, T, max_extend_len, max_seq_len, num_heads, Hkv, D, page_size, window, 0,
-                              dtype_code(q.dtype), D ** -0.5 if scale is None else scale, softcap), current_stream())
-    if code:
-        check(code, "m355_scored_attn")
+    _scored_call("m355_scored_attn", q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ids, lens, pre, cu, out.data_ptr(),
+                 slope_ptr, doc_ptr, bidir_ptr, 0, 0, ws_ptr, q2.stride(0) if T > 1 else W, o_stride, pitch, S, pt_stride, ws_bytes, pt_rows, pt_cols,
+                 B, T, max_extend_len, max_seq_len, num_heads, Hkv, D, page_size, window, 0, dtype_code(q.dtype),
+                 D ** -0.5 if scale is None else scale, softcap)
     return out
 
 
@@ -594,13 +602,10 @@ def tree_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_
     out, o_stride = _out_rows("tree_attn", q2, out, T, W)
     need = 0 if workspace is not None else scored_workspace_bytes(B, T, num_heads, Hkv, D, plan.max_nodes, max_seq_len)
     held, ws_ptr, ws_bytes = _scratch(workspace, need, q.device)
-    code = _lib.load().m355_tree_attn(
-        _lib.SCORED_ARGS.pack(q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ids, 0, pre, cu, out.data_ptr(),
-                              slope_ptr, 0, 0, mask.data_ptr(), pos_ptr, ws_ptr, q2.stride(0) if T > 1 else W, o_stride, pitch, S, pt_stride,
-                              ws_bytes, pt_rows, pt_cols, B, T, plan.max_nodes, max_seq_len, num_heads, Hkv, D, page_size, 0, mask.shape[1],
-                              dtype_code(q.dtype), D ** -0.5 if scale is None else scale, softcap), current_stream())
-    if code:
-        check(code, "m355_tree_attn")
+    _scored_call("m355_tree_attn", q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ids, 0, pre, cu, out.data_ptr(),
+                 slope_ptr, 0, 0, mask.data_ptr(), pos_ptr, ws_ptr, q2.stride(0) if T > 1 else W, o_stride, pitch, S, pt_stride, ws_bytes, pt_rows, pt_cols,
+                 B, T, plan.max_nodes, max_seq_len, num_heads, Hkv, D, page_size, 0, mask.shape[1], dtype_code(q.dtype),
+                 D ** -0.5 if scale is None else scale, softcap)
     return out
 
 

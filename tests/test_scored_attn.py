@@ -341,3 +341,38 @@ def test_refusals():
         c.run(window=-2)
     with pytest.raises(MI355AttnError):
         c.run(scale=0.0)
+    with pytest.raises(MI355AttnError, match="fit"):
+        c.run(window=2 ** 40)
+    with pytest.raises(MI355AttnError):
+        c.run(softcap=1e300)
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, each over its own workspace, with splits and without: every one gives what it gives alone."""
+    cases = [(Case(25, BF, (8, 2, 64), 16, [1500, 40], [1, 1]), dict(decode=True, softcap=30.0)),
+             (Case(26, HF, (4, 1, 128), 16, [900, 5], [60, 33]), dict(window=400))]
+    alone = [c.run(**kw) for c, kw in cases]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(5):
+        for (c, kw), side in zip(cases, sides):
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                got.append(c.run(**kw))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, alone[i % 2]) for i, o in enumerate(got))
+
+
+def test_one_table_row_for_several_requests():
+    """Requests that share a row of the page table: the same tokens, of different lengths."""
+    c = Case(27, BF, (4, 2, 64), 16, [200, 200, 200], [1, 1, 1])
+    c.rows[1:] = c.rows[0]
+    c.len, c.pre = [201, 150, 7], [200, 149, 6]
+    c.slots = [c.slots[0][:n] for n in c.len]
+    check(c.run(decode=True, softcap=30.0), *c.want(softcap=30.0))
+    c.pre, c.ext, c.len, c.cu = [100, 0, 3], [60, 60, 60], [160, 60, 63], [0, 60, 120, 180]
+    c.T = 180
+    c.q = torch.randn((180, 4, 64), generator=c.g).to(BF)
+    c.slots = [([int(c.table[c.rows[0], t // 16]) * 16 + t % 16 for t in range(n)]) for n in c.len]
+    check(c.run(slopes=slopes_of(4).to(DEV)), *c.want(slopes=slopes_of(4)))

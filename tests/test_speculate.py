@@ -62,6 +62,13 @@ def test_dispatch_of_layers_and_masks():
     assert not _any(_masks(SimpleNamespace())) and _any(_masks(SimpleNamespace(doc_starts=torch.zeros(0, dtype=torch.int32), bidir_lens=None)))
 
 
+def test_bench_modes_exclude_each_other():
+    import bench_one_batch as bob
+    for kw in (dict(graph=True, speculate=4), dict(graph=True, top_logprobs=2), dict(speculate=4, top_logprobs=2)):
+        with pytest.raises(ValueError, match="one of"):
+            bob.latency_test(None, bob.BenchArgs(**kw), 1, 8, 4, print, 1)
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 def _engine(heads, ps, lens, dtype=torch.bfloat16, layers=2, extra=200):
     import mi355_attn as m
@@ -223,6 +230,21 @@ def test_trees_refuse_windowed_layers():
         be.forward(z, z[:, :128], z[:, :128], m.Attention(0, 4, 2, 64, window=4), batch)
     batch.commit_tree([[]])
     assert batch.seq_lens_host == [5]
+
+
+@pytest.mark.gpu
+def test_trees_take_no_masks():
+    import mi355_attn as m
+    kv, pm, be, batch = _engine((4, 2, 64), 16, [5])
+    batch.prepare_for_prefill()
+    batch.prepare_for_tree([[1, 2]], [[-1, 0]])
+    batch.doc_starts = torch.zeros(2, dtype=torch.int32, device=DEV)
+    be.init_forward_metadata(batch)
+    z = torch.zeros((2, 4 * 64), dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="mask"):
+        be.forward(z, z[:, :128], z[:, :128], m.Attention(0, 4, 2, 64), batch)
+    batch.commit_tree([[0]])
+    assert batch.doc_starts is None and batch.seq_lens_host == [6]
 
 
 @pytest.mark.gpu

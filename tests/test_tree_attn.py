@@ -174,3 +174,39 @@ def test_refusals():
         prepare(c, [[-1, 0, 1, 2]], new_pages=torch.zeros(1, dtype=torch.int32, device=DEV))
     with pytest.raises(MI355AttnError, match="parents"):
         ops.tree_prepare(c.table.to(DEV), c.rows.to(DEV), torch.tensor([5], device=DEV), torch.zeros(4, device=DEV), plan.cu_q, 16, 4)
+
+
+def test_verification_step_replays_from_a_graph():
+    """Metadata, attention and log probabilities of a step as one graph, replayed over other trees, prefixes and queries."""
+    from mi355_attn import ops
+    c = Case(41, BF, (8, 2, 64), 16, [600, 33, 90], [7, 7, 7])
+    kp, vp, table, rows = c.pool(c.k), c.pool(c.v), c.table.to(DEV), c.rows.to(DEV)
+    pre, cu = torch.tensor(c.pre, device=DEV), torch.tensor(c.cu, dtype=torch.int32, device=DEV)
+    parents = torch.tensor([x for p in trees(1, [7, 7, 7]) for x in p], dtype=torch.int32, device=DEV)
+    q = c.q.reshape(c.T, -1).to(DEV)
+    head = torch.randn((512, 700), generator=c.g).to(DEV).to(BF)
+    logits = torch.zeros((c.T, 700), dtype=BF, device=DEV)
+
+    def step():
+        plan = ops.tree_prepare(table, rows, pre, parents, cu, 16, 7)
+        out = ops.tree_attn(q, kp, vp, table, rows, pre, plan, 16, 8, 700, softcap=20.0)
+        torch.mm(out, head, out=logits)
+        return plan.mask, plan.positions, plan.out_cache_loc, out, *ops.token_logprobs(logits, plan.positions % 700, top_k=3)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for n in range(4):
+        q.copy_(torch.randn(q.shape, generator=c.g).to(BF))
+        pre.copy_(torch.tensor([600 - 97 * n, 33 - 8 * n, 90 - n]))
+        parents.copy_(torch.tensor([x for p in trees(50 + n, [7, 7, 7]) for x in p], dtype=torch.int32))
+        want = [x.clone() for x in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
