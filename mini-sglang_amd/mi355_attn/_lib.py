@@ -162,10 +162,14 @@ _raw_stream = None
 def current_stream() -> int:
     """hipStream_t of torch's current stream on the current device (the stream every entry point launches on).
     torch.cuda.current_stream() costs ~8 us of Python per call; the raw getter is a plain C call."""
-    global _raw_stream
     import torch
+    return stream_of(torch.cuda.current_device())
+
+
+def stream_of(device: int) -> int:
+    """The same for a device whose number the caller holds already: the current one."""
+    global _raw_stream
     if _raw_stream is None:
-        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", False)
-    if _raw_stream:
-        return _raw_stream(torch.cuda.current_device())
-    return torch.cuda.current_stream().cuda_stream
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", False) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+    return _raw_stream(device)

@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from ._lib import check, current_stream, dtype_code, require_cuda
+from ._lib import check, current_stream, dtype_code, require_cuda, stream_of
 
 
 def _ptr(t):
@@ -392,20 +392,22 @@ def rope_kv_store(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, hea
 # ---- attention with modified scores, trees of drafted tokens, log probabilities -----------------------------------------
 # (These calls sit on the path of every layer of every step, so their checks are written for few interpreter steps: a wrapper that
 # took 20 us of host time would be longer than most of the launches behind it.)
-def _on_device(*named) -> None:
-    """Every tensor on the GPU that is current: the launch goes to its stream, and kernels of one device must not be handed
-    another's memory.  `named`: name, tensor, name, tensor, ...; None is skipped."""
-    dev = None
-    for name, t in zip(named[::2], named[1::2]):
-        if t is None:
-            continue
-        at = t.get_device()
-        if at < 0:
+def _on_device(names: str, *tensors) -> int:
+    """The number of the current device, on which every tensor has to be: the launch goes to its stream, and kernels of one device
+    must not be handed another's memory.  `names`: the tensors' names in order; None is skipped."""
+    dev = tensors[0].get_device()
+    if dev >= 0 and dev == torch.cuda.current_device():
+        for t in tensors:
+            if t is not None and t.get_device() != dev:
+                break
+        else:
+            return dev
+    for name, t in zip(names.split(), tensors):
+        if t is not None:
             require_cuda(t, name)
-        if dev is None:
-            dev = torch.cuda.current_device()
-        if at != dev:
-            raise _lib.MI355AttnError(f"{name} is on {t.device}, the current device is cuda:{dev} (use torch.cuda.device)")
+            if t.get_device() != torch.cuda.current_device():
+                raise _lib.MI355AttnError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()} (use torch.cuda.device)")
+    return dev
 
 
 def _vector(name: str, t, dtype, n: int) -> int:
@@ -454,7 +456,7 @@ def _table(what: str, page_table, page_size: int):
 
 def _out_rows(what: str, q, out, T: int, width: int):
     if out is None:
-        return q.new_empty((T, width)), width
+        return torch.empty_like(q, memory_format=torch.contiguous_format), width
     if out.dtype is not q.dtype or out.shape != (T, width) or (T and out.stride(1) != 1):
         raise _lib.MI355AttnError(f"{what}: out must be {q.dtype} [T, heads*D] with inner stride 1")
     if T and out.data_ptr() == q.data_ptr():
@@ -479,14 +481,11 @@ def scored_workspace_bytes(B: int, T: int, Hq: int, Hkv: int, D: int, max_extend
     return int(_lib.load().m355_scored_workspace_bytes(B, T, Hq, Hkv, D, max_extend_len, max_seq_len))
 
 
-def _scored_call(entry: str, *fields) -> None:
+def _scored_args(entry: str, *fields) -> bytes:
     try:
-        args = _lib.SCORED_ARGS.pack(*fields)
+        return _lib.SCORED_ARGS.pack(*fields)
     except struct.error as e:
         raise _lib.MI355AttnError(f"{entry}: an argument does not fit its field: {e}") from None
-    code = getattr(_lib.load(), entry)(args, current_stream())
-    if code:
-        check(code, entry)
 
 
 def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
@@ -504,9 +503,8 @@ def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, pag
     With prefix_lens (int64 [B]) and cu_q (int32 [B+1]): ragged rows over cached prefixes, as prefill_attn; rows of q at or past
     cu_q[B] are left as they were in `out`.  Without them: one row per request, its newest token at seq_lens - 1.  A row that
     sees nothing gives zeros."""
-    _on_device("q", q, "k_pool", k_pool, "v_pool", v_pool, "page_table", page_table, "page_table_ids", page_table_ids, "seq_lens", seq_lens,
-               "prefix_lens", prefix_lens, "cu_q", cu_q, "slopes", slopes, "doc_starts", doc_starts, "bidir_lens", bidir_lens,
-               "workspace", workspace, "out", out)
+    dev = _on_device("q k_pool v_pool page_table page_table_ids seq_lens prefix_lens cu_q slopes doc_starts bidir_lens workspace out",
+                     q, k_pool, v_pool, page_table, page_table_ids, seq_lens, prefix_lens, cu_q, slopes, doc_starts, bidir_lens, workspace, out)
     B, T, max_seq_len, max_extend_len = seq_lens.numel(), q.shape[0], int(max_seq_len), int(max_extend_len)
     S, Hkv, D, pitch = _pools("scored_attn", q, k_pool, v_pool)
     pt_rows, pt_cols, pt_stride = _table("scored_attn", page_table, page_size)
@@ -528,10 +526,13 @@ def scored_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, pag
     out, o_stride = _out_rows("scored_attn", q2, out, T, W)
     need = 0 if workspace is not None else scored_workspace_bytes(B, T, num_heads, Hkv, D, max_extend_len, max_seq_len)
     held, ws_ptr, ws_bytes = _scratch(workspace, need, q.device)
-    _scored_call("m355_scored_attn", q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ids, lens, pre, cu, out.data_ptr(),
+    args = _scored_args("m355_scored_attn", q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ids, lens, pre, cu, out.data_ptr(),
                  slope_ptr, doc_ptr, bidir_ptr, 0, 0, ws_ptr, q2.stride(0) if T > 1 else W, o_stride, pitch, S, pt_stride, ws_bytes, pt_rows, pt_cols,
                  B, T, max_extend_len, max_seq_len, num_heads, Hkv, D, page_size, window, 0, dtype_code(q.dtype),
                  D ** -0.5 if scale is None else scale, softcap)
+    code = _lib.load().m355_scored_attn(args, stream_of(dev))
+    if code:
+        check(code, "m355_scored_attn")
     return out
 
 
@@ -553,8 +554,8 @@ def tree_prepare(page_table: torch.Tensor, page_table_ids: torch.Tensor, prefix_
     """Metadata of a batch of draft trees, one launch (m355_tree_prepare): ancestor masks, positions and slots of all nodes, and
     the page-table entries of new_pages (int32; request b owns new_pages[new_page_off[b]:new_page_off[b+1]], behind the pages of
     its prefix).  parents int32 [T]: index of the parent inside the request, below the node's own, or -1."""
-    _on_device("page_table", page_table, "page_table_ids", page_table_ids, "prefix_lens", prefix_lens, "parents", parents, "cu_q", cu_q,
-               "new_pages", new_pages, "new_page_off", new_page_off)
+    dev = _on_device("page_table page_table_ids prefix_lens parents cu_q new_pages new_page_off",
+                     page_table, page_table_ids, prefix_lens, parents, cu_q, new_pages, new_page_off)
     B, T = prefix_lens.numel(), parents.numel()
     pt_rows, pt_cols, pt_stride = _table("tree_prepare", page_table, page_size)
     ids, pre = _vector("page_table_ids", page_table_ids, torch.int64, B), _vector("prefix_lens", prefix_lens, torch.int64, B)
@@ -573,7 +574,7 @@ def tree_prepare(page_table: torch.Tensor, page_table_ids: torch.Tensor, prefix_
     mask = parents.new_empty((T, words))
     positions, slots = prefix_lens.new_empty((2, T)).unbind()
     code = _lib.load().m355_tree_prepare(page_table.data_ptr(), pt_stride, pt_rows, pt_cols, ids, pre, par, cu, fresh, off, n, B, T, max_nodes,
-                                         page_size, mask.data_ptr(), words, positions.data_ptr(), slots.data_ptr(), current_stream())
+                                         page_size, mask.data_ptr(), words, positions.data_ptr(), slots.data_ptr(), stream_of(dev))
     if code:
         check(code, "m355_tree_prepare")
     return TreePlan(mask, positions, slots, cu_q, max_nodes)
@@ -587,8 +588,8 @@ def tree_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_
     written to plan.out_cache_loc.  max_seq_len >= the longest prefix + nodes; softcap / slopes as scored_attn, distances between
     nodes being differences of depth."""
     mask, positions, cu_q = plan.mask, plan.positions, plan.cu_q
-    _on_device("q", q, "k_pool", k_pool, "v_pool", v_pool, "page_table", page_table, "page_table_ids", page_table_ids, "prefix_lens", prefix_lens,
-               "mask", mask, "positions", positions, "cu_q", cu_q, "slopes", slopes, "workspace", workspace, "out", out)
+    dev = _on_device("q k_pool v_pool page_table page_table_ids prefix_lens mask positions cu_q slopes workspace out",
+                     q, k_pool, v_pool, page_table, page_table_ids, prefix_lens, mask, positions, cu_q, slopes, workspace, out)
     B, T, max_seq_len = prefix_lens.numel(), q.shape[0], int(max_seq_len)
     S, Hkv, D, pitch = _pools("tree_attn", q, k_pool, v_pool)
     pt_rows, pt_cols, pt_stride = _table("tree_attn", page_table, page_size)
@@ -602,10 +603,13 @@ def tree_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_
     out, o_stride = _out_rows("tree_attn", q2, out, T, W)
     need = 0 if workspace is not None else scored_workspace_bytes(B, T, num_heads, Hkv, D, plan.max_nodes, max_seq_len)
     held, ws_ptr, ws_bytes = _scratch(workspace, need, q.device)
-    _scored_call("m355_tree_attn", q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ids, 0, pre, cu, out.data_ptr(),
+    args = _scored_args("m355_tree_attn", q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ids, 0, pre, cu, out.data_ptr(),
                  slope_ptr, 0, 0, mask.data_ptr(), pos_ptr, ws_ptr, q2.stride(0) if T > 1 else W, o_stride, pitch, S, pt_stride, ws_bytes, pt_rows, pt_cols,
                  B, T, plan.max_nodes, max_seq_len, num_heads, Hkv, D, page_size, 0, mask.shape[1], dtype_code(q.dtype),
                  D ** -0.5 if scale is None else scale, softcap)
+    code = _lib.load().m355_tree_attn(args, stream_of(dev))
+    if code:
+        check(code, "m355_tree_attn")
     return out
 
 
@@ -620,7 +624,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
                    workspace: Optional[torch.Tensor] = None) -> TokenLogprobs:
     """Log probabilities of `tokens` (int64 [T] or [T, n]; None: none) under softmax(logits / temperature), the rows' entropies
     and their top_k alternatives, ties to the lower id, in one pass over logits [T, V] (m355_token_logprobs)."""
-    _on_device("logits", logits, "tokens", tokens, "workspace", workspace)
+    on = _on_device("logits tokens workspace", logits, tokens, workspace)
     if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1 and logits.shape[1] > 1):
         raise _lib.MI355AttnError(f"token_logprobs: logits must be [T, V] with inner stride 1, got {tuple(logits.shape)}")
     T, V = logits.shape
@@ -644,7 +648,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     held, ws_ptr, ws_bytes = _scratch(workspace, 0 if workspace is not None else _logprobs_workspace_bytes(T, V, top_k), dev)
     code = _lib.load().m355_token_logprobs(logits.data_ptr(), logits.stride(0) if T > 1 else V, tok_ptr, given, T, V, top_k, temperature, lp_ptr,
                                            entropy.data_ptr(), top.data_ptr(), ids.data_ptr(), ws_ptr, ws_bytes, dtype_code(logits.dtype),
-                                           current_stream())
+                                           stream_of(on))
     if code:
         check(code, "m355_token_logprobs")
     return TokenLogprobs(lp, entropy, top, ids)
