@@ -66,7 +66,7 @@ def speculative_decode(runner, next_ids: torch.Tensor, batch, new_tokens: int, n
     logprobs: List[List[float]] = [[] for _ in first]
     steps = 0
     while min(len(o) for o in out) < new_tokens:
-        # (a request that is done keeps verifying its own last token until the batch is: the batch stays as it is)
+        # (a request that is done stays in the batch with its last token as a tree of one, of which nothing is kept)
         trees = [draft(h, max(1, min(nodes, new_tokens - len(o)))) for h, o in zip(history, out)]
         batch.prepare_for_tree([t for t, _ in trees], [p for _, p in trees])
         logits, _ = runner.forward(batch)
@@ -75,7 +75,7 @@ def speculative_decode(runner, next_ids: torch.Tensor, batch, new_tokens: int, n
         paths, at = [], 0
         for b, tree in enumerate(trees):
             n = len(tree[0])
-            path = accepted_path(tree, best[at:at + n])
+            path = accepted_path(tree, best[at:at + n]) if len(out[b]) < new_tokens else []
             got = [best[at + node] for node in path]
             history[b] += got
             out[b] += got

@@ -314,7 +314,8 @@ class Batch:
 
     def commit_tree(self, accepted: List[List[int]]) -> None:
         """Ends a verification step: request b keeps the nodes accepted[b], a path from a root downwards (may be empty).  Their
-        K/V move to the slots of their positions, the other nodes' pages go back to the pool, the lengths grow by the paths."""
+        K/V move to the slots of their positions, the other nodes' pages go back to the pool, the lengths grow by the paths.  A
+        prepare_for_decode that follows wants output_ids set: the tokens sampled last, which are not cached yet."""
         if self.tree is None:
             raise RuntimeError("commit_tree: no tree is open")
         for path, par in zip(accepted, self._tree_parents):

@@ -69,6 +69,46 @@ def test_bench_modes_exclude_each_other():
             bob.latency_test(None, bob.BenchArgs(**kw), 1, 8, 4, print, 1)
 
 
+def test_a_request_that_is_done_keeps_nothing_more(monkeypatch):
+    """Requests of a batch advance at their own pace: one that has its tokens must not fill the cache while the others go on."""
+    from types import SimpleNamespace
+
+    from harness import speculate
+    nxt = lambda t: (7 * t + 3) % 50  # noqa: E731
+    kept, held = [0, 0], []
+
+    class FakeBatch:
+        reqs = [SimpleNamespace(origin_input_ids=[1, 2]), SimpleNamespace(origin_input_ids=[5])]
+
+        def prepare_for_tree(self, ids, parents):
+            self.ids = ids
+            held.append([k + len(i) for k, i in zip(kept, ids)])
+
+        def commit_tree(self, paths):
+            for b, path in enumerate(paths):
+                kept[b] += len(path)
+
+    def logprobs(logits, top_k):
+        return SimpleNamespace(top_ids=logits.argmax(1, keepdim=True), top_logprobs=logits.max(1, keepdim=True).values)
+
+    monkeypatch.setattr(speculate.m.ops, "token_logprobs", logprobs)
+    forward = lambda batch: (torch.nn.functional.one_hot(torch.tensor([nxt(t) for i in batch.ids for t in i]), 50).float(), None)  # noqa: E731
+
+    def draft(history, nodes):
+        chain = [history[-1]]
+        while history[0] == 1 and len(chain) < nodes:                      # the first request's drafts are all right
+            chain.append(nxt(chain[-1]))
+        return chain, list(range(-1, len(chain) - 1))
+
+    out, lps, steps = speculate.speculative_decode(SimpleNamespace(forward=forward), torch.tensor([4, 6]), FakeBatch(), 10, 5, draft)
+    for ids, first in zip(out, (4, 6)):
+        want = [nxt(first)]
+        while len(want) < 10:
+            want.append(nxt(want[-1]))
+        assert ids == want
+    assert steps == 10 and kept == [10, 10] and max(max(h) for h in held) <= 11 and all(len(x) == 10 for x in lps)
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 def _engine(heads, ps, lens, dtype=torch.bfloat16, layers=2, extra=200):
     import mi355_attn as m
