@@ -308,8 +308,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
 // 4 D matrix flops; a cap puts two more transcendentals and two plain instructions on top.  A prompt of 8192 tokens (32 / 8 heads of
 // 128): 590 us plain, 930 TFLOP/s, 700 capped (capping one tile beside the other's matrix product in source order, forced or
 // not: within 1%; the SIMD's other wave already fills the gaps).  16 capped turns of 384 to 640 tokens over 1024 cached: 275
-// us, 635 TFLOP/s, in four rounds of workgroups the last of which is partly empty.  Documents of ~700 tokens at head_dim 64: 128 us, 470
-// TFLOP/s, half the matrix work per score and some nine key pairs a block, of which the first and last are masked.  Eight waves a workgroup
+// us, 635 TFLOP/s, in four rounds of workgroups the last of which is partly empty.  Documents of ~700 tokens at head_dim 64: 129 us, 470
+// TFLOP/s against 780 without documents: some nine key pairs a block, of which the first and last are masked, and the block's start.  Eight waves a workgroup
 // (256 rows) gained nothing.
 // ------------------------------------------------------------------------------------------------------------------------
 template <int D, bool MOD, bool F16, bool SPLIT>
