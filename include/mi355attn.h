@@ -258,8 +258,9 @@ int m355_rope_kv_store(void *q, int64_t q_row_stride, void *k, int64_t k_row_str
  * (rows at or past cu_q[B] are left alone); both NULL - one row per request, its newest token at seq_lens[b] - 1 (a request of
  * length 0 gives zeros).
  * m355_tree_attn: row cu_q[b] + j is node j of request b's draft tree (m355_tree_prepare); it sees the prefix_lens[b] cached tokens
- * and the nodes of its mask row, whose K/V are in the pools already.  Distances between nodes are differences of depth: positions is
- * read for the bias only and may be NULL without slopes.  seq_lens, window, doc_starts and bidir_lens must be NULL / 0.
+ * and the nodes of its mask row, whose K/V are in the pools already, of these the ones whose positions its window holds.  Distances
+ * between nodes are differences of depth: positions (prefix + depth) is read for bias and window and may be NULL without both.
+ * seq_lens, doc_starts and bidir_lens must be NULL.
  * A row that sees nothing - its mask is empty, or every visible score is -inf - gives zeros.  What masked keys and values hold
  * never reaches an output, infinities and NaN included.  Any Hq that is a multiple of Hkv; head_dim 64 or 128; bf16 or fp16.
  * Whatever the tables hold, nothing outside the pools, the table and the T rows is read: ids and pages out of range are brought

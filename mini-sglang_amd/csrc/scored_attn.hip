@@ -5,7 +5,7 @@
 //     out[t]  = sum_k softmax(x[t, .])_k V[k]  over the visible keys of row t;  zeros where the mask leaves nothing
 //
 // visible: an interval (causal, window, document start, bidirectional prefix: scored_rules.h visible_range) or, for a tree of
-// drafted tokens, the prefix and the row's ancestors (tree_bits).
+// drafted tokens, the prefix and the row's ancestors (tree_bits), inside a window of positions.
 //
 // A query row is a (token, q head of the group) pair, token-major, so the G heads that share a kv head share its loads.  Two
 // kernels, by the rows a request brings: scored_few_kernel (single tokens: HBM-bound) and scored_wide_kernel (long
@@ -61,6 +61,8 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 constexpr int kFewRows = 16, kFewWaves = 2, kWideRows = 128;
 constexpr int kFewSlots = 1024;                       // tokens whose pool slots are in LDS at a time
 
+enum { kPlain, kCapped, kBiased };                         // what scores go through: the scale alone, a cap, distances (capped or not)
+
 template <int D, bool MOD, bool F16>
 __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const ScoredParams p) {
     using M = MG<D>;
@@ -86,7 +88,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
     int32_t lo = 0, hi = r.L, pos = r.P + j;
     BlockRange br;
     if (p.mask) {
-        if (MOD && p.slopes) pos = (int32_t)p.positions[t];
+        if ((MOD && p.slopes) || p.window) pos = (int32_t)p.positions[t];
+        lo = tree_lo(p, r, pos);
     } else {
         const KeyRange v = visible_range(pos, r.L, p.window, p.doc_starts ? p.doc_starts[t] : 0, p.bidir ? p.bidir[b] : 0);
         lo = v.lo; hi = v.hi;
@@ -194,10 +197,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
             const uint32_t w = bits >> (4 * kg);
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[i] = masked_score(s[i], w, 16 * (i >> 2) + (i & 3));
-            uint32_t carry = 0;
+            Extremes of;
 #pragma unroll
-            for (int dt = 0; dt < M::DT; ++dt) carry |= frag_carry<F16>(v_frag(st, dt));
-            bad = any_nonfinite(carry);
+            for (int dt = 0; dt < M::DT; ++dt) of.add(v_frag(st, dt));
+            bad = of.nonfinite();
         }
         float mx = s[0], a, c;
 #pragma unroll
@@ -304,15 +307,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
 // those of prefill_attn.hip (v_mfma_f32_32x32x16, a lane owns one row and 16 of a tile's keys); what differs is the score
 // stage between them and the range that is walked.
 //
-// Bound by vector issue: per score a multiply-add, an exponential, a sum, half a maximum and a quarter of a conversion stand beside
+// Bound by vector issue: per score a multiply-add, an exponential, a sum, half a maximum and half a conversion stand beside
 // 4 D matrix flops; a cap puts two more transcendentals and two plain instructions on top.  A prompt of 8192 tokens (32 / 8 heads of
-// 128): 590 us plain, 930 TFLOP/s, 700 capped (capping one tile beside the other's matrix product in source order, forced or
-// not: within 1%; the SIMD's other wave already fills the gaps).  16 capped turns of 384 to 640 tokens over 1024 cached: 275
-// us, 635 TFLOP/s, in four rounds of workgroups the last of which is partly empty.  Documents of ~700 tokens at head_dim 64: 129 us, 470
-// TFLOP/s against 780 without documents: some nine key pairs a block, of which the first and last are masked, and the block's start.  Eight waves a workgroup
-// (256 rows) gained nothing.
+// 128): 590 us plain, 930 TFLOP/s, 694 capped (capping one tile beside the other's matrix product in source order, forced or
+// not: within 1%; the SIMD's other wave already fills the gaps).  16 capped turns of 384 to 640 tokens over 1024 cached: 273
+// us, 640 TFLOP/s, in four rounds of workgroups the last of which is partly empty.  Documents of ~700 tokens at head_dim 64: 127 us,
+// 475 TFLOP/s against 780 without documents: some nine key pairs a block, of which the first and last are masked, and the
+// block's start.  Eight waves a workgroup (256 rows) gained nothing.  Capped scores have a kernel apart from biased ones: in one, the
+// registers of both spill at head_dim 128 (16 capped turns 279 us, 4 trees of 64 nodes over 20 000 to 32 000 tokens 59 for 53).
 // ------------------------------------------------------------------------------------------------------------------------
-template <int D, bool MOD, bool F16, bool SPLIT>
+template <int D, int MOD, bool F16, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams p) {
     using W = WgCfg<D>;
     constexpr int NW = 4, NBUF = 4;
@@ -358,7 +362,8 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     int32_t pos = r.P + j, lo = 0, hi = r.L;
     BlockRange br = {0x7fffffff, 0, 0, 0x7fffffff};                // the wave's rows
     if (p.mask) {
-        if (MOD && p.slopes) pos = (int32_t)p.positions[t];
+        if (MOD == kBiased || p.window) pos = (int32_t)p.positions[t];
+        lo = tree_lo(p, r, pos);
     } else {
         const KeyRange v = visible_range(pos, r.L, p.window, p.doc_starts ? p.doc_starts[t] : 0, p.bidir ? p.bidir[b] : 0);
         lo = v.lo; hi = v.hi;
@@ -396,8 +401,8 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     }
     // a score in log2 units is unit * s, s being what `modify` leaves: a capped one is kept as -1 / (1 + e^2x), which is its tanh but for
     // a factor and a constant; the constant drops out of the softmax and the factor into the exponent's multiply-add
-    const float unit = !MOD ? p.scale_log2 : p.cap_log2 > 0.f ? 2.f * p.cap_log2 : 1.f;
-    const float slope = MOD && p.slopes ? p.slopes[h * p.G + g] * kLog2e / unit : 0.f;
+    const float unit = MOD == kPlain ? p.scale_log2 : MOD == kCapped || p.cap_log2 > 0.f ? 2.f * p.cap_log2 : 1.f;
+    const float slope = MOD == kBiased ? p.slopes[h * p.G + g] * kLog2e / unit : 0.f;
     int lo_wg, hi_wg;
     if (p.doc_starts) {
         __syncthreads();
@@ -479,14 +484,14 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     };
     // lane: keys base + (i & 3) + 8 (i >> 2) + 4 hh
     auto modify = [&](f32x16& s, const int base) {
-        if (p.cap_log2 > 0.f) {
+        if (MOD == kCapped || p.cap_log2 > 0.f) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_rcpf(-1.f - exp2_fast(s[i] * p.cap_rate));
         } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] *= p.scale_log2;
         }
-        if (p.slopes) {
+        if constexpr (MOD == kBiased) {
             if (p.mask && base + 32 > r.P) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -545,10 +550,10 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
     };
     // infinities and NaN of a tile's V fragments: out of the product, into the rows that see them
     auto clean = [&](bf16x8 (&f)[W::KS], const int buf, const uint32_t bits) {
-        uint32_t carry = 0;
+        Extremes of;
 #pragma unroll
-        for (int s = 0; s < W::KS; ++s) carry |= frag_carry<F16>(f[s]);
-        if (!any_nonfinite(carry)) return;
+        for (int s = 0; s < W::KS; ++s) of.add(f[s]);
+        if (!of.nonfinite()) return;
 #pragma unroll
         for (int s = 0; s < W::KS; ++s) f[s] = frag_finite<F16>(f[s]);
         for (int tk = 0; tk < 32; ++tk) {
@@ -603,7 +608,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int x = 0; x < IPW; ++x) piece(false, x, sl[x], nb);
-        if constexpr (MOD) { modify(sa, base_a); modify(sb, base_b); }
+        if constexpr (MOD != kPlain) { modify(sa, base_a); modify(sb, base_b); }
         const bool part = base_a < w_lo_max || base_a + 64 > w_hi_min;      // wave-uniform
         uint32_t bits_a = 0, bits_b = 0;
         if (part) {
@@ -820,13 +825,13 @@ static void launch_merge(const ScoredParams& p, int64_t rows, hipStream_t st) {
     else hipLaunchKernelGGL((scored_merge_kernel<D, RB, 1, F16>), dim3((unsigned)((rows * LPI + 255) / 256)), dim3(256), 0, st, p);
 }
 
-template <int D, bool MOD, bool F16>
+template <int D, int MOD, bool F16>
 static void launch_kernels(const ScoredParams& p, const ScoredCut& c, hipStream_t st) {
     if (c.wide) {
         if (p.slots) hipLaunchKernelGGL((scored_wide_kernel<D, MOD, F16, true>), dim3((unsigned)c.grid), dim3(256), 0, st, p);
         else hipLaunchKernelGGL((scored_wide_kernel<D, MOD, F16, false>), dim3((unsigned)c.grid), dim3(256), 0, st, p);
     } else {
-        hipLaunchKernelGGL((scored_few_kernel<D, MOD, F16>), dim3((unsigned)c.grid), dim3(64 * kFewWaves), 0, st, p);
+        hipLaunchKernelGGL((scored_few_kernel<D, MOD != kPlain, F16>), dim3((unsigned)c.grid), dim3(64 * kFewWaves), 0, st, p);
     }
     if (p.slots) {
         const int64_t rows = (int64_t)p.T * p.Hq;
@@ -854,10 +859,13 @@ static int launch_scored(const M355ScoredArgs& a, void* stream) {
     p.blocks = c.blocks; p.slots = c.slots; p.max_parts = c.max_parts;
     if (c.bytes) { p.part = (float*)a.workspace; p.part_of = (int2*)((uint8_t*)a.workspace + c.part_bytes); }
     hipStream_t st = (hipStream_t)stream;
-    const bool mod = a.softcap > 0.f || a.slopes, f16 = a.dtype == M355_DTYPE_F16;
+    const int mod = a.slopes ? kBiased : a.softcap > 0.f ? kCapped : kPlain;
+    const bool f16 = a.dtype == M355_DTYPE_F16;
 #define M355_SCORED(DD, MM, FF) if (a.D == DD && mod == MM && f16 == FF) { launch_kernels<DD, MM, FF>(p, c, st); return check_launch(); }
-    M355_SCORED(64, false, false) M355_SCORED(64, false, true) M355_SCORED(64, true, false) M355_SCORED(64, true, true)
-    M355_SCORED(128, false, false) M355_SCORED(128, false, true) M355_SCORED(128, true, false) M355_SCORED(128, true, true)
+    M355_SCORED(64, kPlain, false) M355_SCORED(64, kCapped, false) M355_SCORED(64, kBiased, false)
+    M355_SCORED(64, kPlain, true) M355_SCORED(64, kCapped, true) M355_SCORED(64, kBiased, true)
+    M355_SCORED(128, kPlain, false) M355_SCORED(128, kCapped, false) M355_SCORED(128, kBiased, false)
+    M355_SCORED(128, kPlain, true) M355_SCORED(128, kCapped, true) M355_SCORED(128, kBiased, true)
 #undef M355_SCORED
     return M355_ERR_UNSUPPORTED;
 }
@@ -886,6 +894,6 @@ extern "C" int m355_tree_attn(const M355ScoredArgs* args, void* stream) {
     const M355ScoredArgs& a = *args;
     if (a.T == 0 || a.B == 0) return M355_OK;
     if (!a.prefix_lens || !a.cu_q || !a.tree_mask || a.mask_words <= 0 || (int64_t)a.mask_words * 32 < a.max_extend_len) return M355_ERR_INVALID_ARG;
-    if (a.seq_lens || a.window || a.doc_starts || a.bidir_lens || (a.slopes && !a.positions)) return M355_ERR_INVALID_ARG;
+    if (a.seq_lens || a.doc_starts || a.bidir_lens || ((a.slopes || a.window) && !a.positions)) return M355_ERR_INVALID_ARG;
     return launch_scored(a, stream);
 }

@@ -21,7 +21,7 @@ struct ScoredParams {
     const int32_t *doc_starts, *bidir;                        // [T], [B], or null
     const uint32_t* mask;                                     // trees: [T, words] ancestor bits; null otherwise
     int32_t words;
-    const int64_t* positions;                                 // trees: position of every node (read when slopes are given)
+    const int64_t* positions;                                 // trees: position of every node (read for slopes and windows)
     // the launch: row blocks of the longest request, and - where keys are split - the workgroups that fit the chip at once, the
     // parts there is room for, and the parts themselves
     int32_t blocks, slots, max_parts;                         // slots 0: no splits
@@ -95,7 +95,7 @@ __device__ __forceinline__ Share find_share(const ScoredParams& p) {
         q.r = load_span(p, at);
         q.row = (int32_t)(row < 0 ? 0 : (row >= p.pt_rows ? p.pt_rows - 1 : row));
         q.blocks = b < p.B ? (q.r.E * p.G + RB - 1) / RB : 0;
-        q.keys = p.window > 0 ? imin(q.r.L, imin(p.window, 0x3fffffff) + RB) : q.r.L;
+        q.keys = p.window > 0 ? imin(q.r.L, imin(p.window, 0x3fffffff) + (p.mask ? q.r.E : RB)) : q.r.L;
         return q;
     };
     const Req first = load(lane);
@@ -158,15 +158,30 @@ struct BlockRange { int32_t lo_min, hi_max, lo_max, hi_min; };
 // Rows j0 .. j1 of a request.  Without documents both limits grow with the row, so the first and the last row tell; a tree's
 // rows all see the prefix and at most the whole tree.
 __device__ __forceinline__ BlockRange block_range(const ScoredParams& p, const ReqSpan& r, int b, int j0, int j1) {
-    if (p.mask) return {0, r.L, 0, imin(r.P, r.L)};
+    if (p.mask) {                                      // positions P .. P + E - 1, in no order
+        if (p.window == 0) return {0, r.L, 0, imin(r.P, r.L)};
+        return {imax(r.P - p.window + 1, 0), r.L, imax(r.P + r.E - p.window, 0), imin(r.P, r.L)};
+    }
     const int32_t bd = p.bidir ? p.bidir[b] : 0;
     const KeyRange a = visible_range(r.P + j0, r.L, p.window, 0, bd), z = visible_range(r.P + j1, r.L, p.window, 0, bd);
     return {a.lo, z.hi, z.lo, a.hi};
 }
 
+// the first token of a tree's prefix that a node at position pos sees; beyond P where the window ends inside the tree
+__device__ __forceinline__ int32_t tree_lo(const ScoredParams& p, const ReqSpan& r, int32_t pos) {
+    return p.window > 0 ? imax(imin(imax(pos, r.P), r.P + r.E - 1) - p.window + 1, 0) : 0;
+}
+
 // bits of the keys of a 32-key tile that a row sees
 __device__ __forceinline__ uint32_t row_bits(const ScoredParams& p, const ReqSpan& r, int64_t t, int32_t lo, int32_t hi, int32_t base) {
-    return p.mask ? tree_bits(p.mask + t * p.words, p.words, r.P, hi, base) : range_bits(lo, hi, base);
+    if (!p.mask) return range_bits(lo, hi, base);
+    uint32_t bits = tree_bits(p.mask + t * p.words, p.words, r.P, hi, base) & ~low_bits(imin(lo, r.P) - base);
+    if (lo > r.P)                                      // the window ends inside the tree: it counts positions, not nodes
+        for (uint32_t left = bits; left; left &= left - 1) {
+            const int k = __builtin_ctz(left);
+            if (p.positions[r.q0 + (base + k - r.P)] < lo) bits &= ~(1u << k);
+        }
+    return bits;
 }
 
 // cap tanh(scale s / cap) log2(e) from the raw product s: tanh(x) = 1 - 2 / (1 + e^2x), exact at both ends (e^2x = 0 and inf);
@@ -184,12 +199,25 @@ __device__ __forceinline__ uint32_t exponent_carry(uint32_t w) {
 }
 template <bool F16>
 __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) { return ((exponent_carry<F16>(w) >> 15) & 0x00010001u) * 0xffffu; }
-template <bool F16>
-__device__ __forceinline__ uint32_t frag_carry(bf16x8 f) {
-    const u32x4 w = __builtin_bit_cast(u32x4, f);
-    return exponent_carry<F16>(w[0]) | exponent_carry<F16>(w[1]) | exponent_carry<F16>(w[2]) | exponent_carry<F16>(w[3]);
-}
-__device__ __forceinline__ bool any_nonfinite(uint32_t carry) { return __any((carry & 0x80008000u) != 0); }
+// Whether fragments hold any, at one instruction a dword: their greatest and least value, read as halves, in the order that NaN leads.  A
+// bf16 infinity or NaN is a NaN as a half, and so are finite values from 2^121 up, for which the caller merely looks closer.
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+struct Extremes {
+    f16x2 hi = {0, 0}, lo = {0, 0};
+    __device__ __forceinline__ void add(bf16x8 f) {
+        const u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const uint32_t x = w[i], y = w[i + 1];     // (__builtin_bit_cast of w[i] itself would take element 0)
+            const f16x2 a = __builtin_bit_cast(f16x2, x), b = __builtin_bit_cast(f16x2, y);
+            hi = __builtin_elementwise_maximum(__builtin_elementwise_maximum(hi, a), b);
+            lo = __builtin_elementwise_minimum(__builtin_elementwise_minimum(lo, a), b);
+        }
+    }
+    __device__ __forceinline__ bool nonfinite() const {                  // in any lane of the wave
+        return __any(((exponent_carry<true>(__builtin_bit_cast(uint32_t, hi)) | exponent_carry<true>(__builtin_bit_cast(uint32_t, lo))) & 0x80008000u) != 0);
+    }
+};
 template <bool F16>
 __device__ __forceinline__ bf16x8 frag_finite(bf16x8 f) {
     u32x4 w = __builtin_bit_cast(u32x4, f);

@@ -225,9 +225,6 @@ class MI355AttnBackend:
             self.init_forward_metadata(batch)
             md = self.forward_metadata
             md.first_layer = layer.layer_id
-        mods = _modifiers(layer)
-        if mods.pop("window"):
-            raise ops._lib.MI355AttnError("MI355AttnBackend: draft trees are not supported in layers with a window")
         if _any(_masks(batch)):
             raise ops._lib.MI355AttnError("MI355AttnBackend: draft trees take no document or prefix mask")
         self._store_kv(k, v, layer, batch)
@@ -235,7 +232,7 @@ class MI355AttnBackend:
         need = ops.scored_workspace_bytes(batch.seq_lens.numel(), q.shape[0], layer.num_heads, layer.num_kv_heads, layer.head_dim,
                                           batch.tree.max_nodes, md.max_seq_len)
         return ops.tree_attn(q, k_pool, v_pool, batch.page_manager.page_table, batch.page_table_ids, batch.seq_lens, batch.tree, self.page_size,
-                             layer.num_heads, md.max_seq_len, workspace=self._ws(need, q.device), **mods)
+                             layer.num_heads, md.max_seq_len, workspace=self._ws(need, q.device), **_modifiers(layer))
 
     def forward_extend(self, q, k, v, layer, batch):
         md = self.forward_metadata

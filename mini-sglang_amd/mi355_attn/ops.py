@@ -582,11 +582,11 @@ def tree_prepare(page_table: torch.Tensor, page_table_ids: torch.Tensor, prefix_
 
 def tree_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
               page_table_ids: torch.Tensor, prefix_lens: torch.Tensor, plan: TreePlan, page_size: int, num_heads: int,
-              max_seq_len: int, *, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, scale: Optional[float] = None,
-              workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+              max_seq_len: int, *, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, window: int = 0,
+              scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of drafted nodes over the cached prefix and their ancestors (m355_tree_attn), after the nodes' K/V have been
-    written to plan.out_cache_loc.  max_seq_len >= the longest prefix + nodes; softcap / slopes as scored_attn, distances between
-    nodes being differences of depth."""
+    written to plan.out_cache_loc.  max_seq_len >= the longest prefix + nodes; softcap / slopes / window as scored_attn, distances
+    between nodes being differences of depth."""
     mask, positions, cu_q = plan.mask, plan.positions, plan.cu_q
     dev = _on_device("q k_pool v_pool page_table page_table_ids prefix_lens mask positions cu_q slopes workspace out",
                      q, k_pool, v_pool, page_table, page_table_ids, prefix_lens, mask, positions, cu_q, slopes, workspace, out)
@@ -605,7 +605,7 @@ def tree_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_
     held, ws_ptr, ws_bytes = _scratch(workspace, need, q.device)
     args = _scored_args("m355_tree_attn", q2.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ids, 0, pre, cu, out.data_ptr(),
                  slope_ptr, 0, 0, mask.data_ptr(), pos_ptr, ws_ptr, q2.stride(0) if T > 1 else W, o_stride, pitch, S, pt_stride, ws_bytes, pt_rows, pt_cols,
-                 B, T, plan.max_nodes, max_seq_len, num_heads, Hkv, D, page_size, 0, mask.shape[1], dtype_code(q.dtype),
+                 B, T, plan.max_nodes, max_seq_len, num_heads, Hkv, D, page_size, window, mask.shape[1], dtype_code(q.dtype),
                  D ** -0.5 if scale is None else scale, softcap)
     code = _lib.load().m355_tree_attn(args, stream_of(dev))
     if code:

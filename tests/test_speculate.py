@@ -259,17 +259,30 @@ def test_tree_step_then_commit_then_decode(ps):
 
 
 @pytest.mark.gpu
-def test_trees_refuse_windowed_layers():
+def test_trees_in_windowed_layers():
     import mi355_attn as m
-    kv, pm, be, batch = _engine((4, 2, 64), 16, [5])
+    Hq, Hkv, D, ps, W = 4, 2, 64, 16, 12
+    kv, pm, be, batch = _engine((Hq, Hkv, D), ps, [40])
+    layer, g = m.Attention(0, Hq, Hkv, D, window=W, logit_cap=15.0), torch.Generator().manual_seed(8)
     batch.prepare_for_prefill()
-    batch.prepare_for_tree([[1, 2]], [[-1, 0]])
     be.init_forward_metadata(batch)
-    z = torch.zeros((2, 4 * 64), dtype=torch.bfloat16, device=DEV)
-    with pytest.raises(RuntimeError, match="window"):
-        be.forward(z, z[:, :128], z[:, :128], m.Attention(0, 4, 2, 64, window=4), batch)
-    batch.commit_tree([[]])
-    assert batch.seq_lens_host == [5]
+    qkv = _rand(g, 40, Hq, Hkv, D)
+    be.forward(*(t for t in qkv.to(DEV).split([Hq * D, Hkv * D, Hkv * D], dim=-1)), layer, batch)
+    parents = [[*range(-1, 14), 3, 15, 0]]                                  # a chain longer than the window, two branches
+    batch.prepare_for_tree([[7] * 18], parents)
+    be.init_forward_metadata(batch)
+    new = _rand(g, 18, Hq, Hkv, D)
+    got = be.forward(*(t for t in new.to(DEV).split([Hq * D, Hkv * D, Hkv * D], dim=-1)), layer, batch).double().cpu().view(18, Hq, D)
+    both = torch.cat([qkv, new])
+    seen, depth = ancestors_ref(parents[0])
+    rows = []
+    for j in range(18):
+        keys = [(k, k) for k in range(40)] + [(40 + x, 40 + depth[x]) for x in sorted(seen[j])]
+        keys = [(k, pos) for k, pos in keys if pos > 40 + depth[j] - W]
+        rows.append(([k for k, _ in keys], [pos for _, pos in keys], 40 + depth[j]))
+    want, tol = attend_ref(new[:, : Hq * D].view(18, Hq, D), both[:, Hq * D:(Hq + Hkv) * D].view(58, Hkv, D), both[:, (Hq + Hkv) * D:].view(58, Hkv, D),
+                           range(58), rows, torch.bfloat16, D ** -0.5, 15.0)
+    assert bool(((got - want).abs() <= tol).all())
 
 
 @pytest.mark.gpu
@@ -288,7 +301,7 @@ def test_trees_take_no_masks():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("model,ps", [("tiny", 16), ("tiny-capped", 4), ("tiny128", 1)])
+@pytest.mark.parametrize("model,ps", [("tiny", 16), ("tiny-capped", 4), ("tiny128", 1), ("tiny-window", 16)])
 def test_speculative_decode_runs_and_agrees(model, ps):
     """Drafts that are right (the plain loop's own tokens, among wrong ones): few steps, the plain loop's tokens, and log
     probabilities that are those of its logits."""

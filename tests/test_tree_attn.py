@@ -35,7 +35,7 @@ def attn(c, plan, **kw):
                          torch.tensor(c.pre, dtype=torch.int64, device=DEV), plan, c.ps, c.Hq, max(c.len), **kw)
 
 
-def want(c, parents, softcap=0.0, slopes=None):
+def want(c, parents, softcap=0.0, slopes=None, window=0):
     outs, tols = [], []
     for b, par in enumerate(parents):
         seen, depth = ancestors_ref(par)
@@ -43,7 +43,9 @@ def want(c, parents, softcap=0.0, slopes=None):
         rows = []
         for j in range(len(par)):
             up = sorted(seen[j])
-            rows.append((list(range(P)) + [P + x for x in up], list(range(P)) + [P + depth[x] for x in up], P + depth[j]))
+            keys = [(k, k) for k in range(P)] + [(P + x, P + depth[x]) for x in up]                    # token, position
+            keys = [(k, pos) for k, pos in keys if not window or pos > P + depth[j] - window]
+            rows.append(([k for k, _ in keys], [pos for _, pos in keys], P + depth[j]))
         o, t = attend_ref(c.q[a:a + len(par)], c.k, c.v, c.slots[b], rows, c.dtype, c.D ** -0.5, softcap, slopes)
         outs.append(o), tols.append(t)
     return torch.cat(outs), torch.cat(tols)
@@ -130,6 +132,26 @@ def test_tree_attention(dtype, heads, ps, pre, ext, mod):
     got = attn(c, prepare(c, parents), **kw)
     check(got, *ref)
     assert torch.equal(got, attn(c, prepare(c, parents), **kw))
+
+
+@pytest.mark.parametrize("window", [1, 3, 20, 64, 333, 2 ** 31 - 1])
+@pytest.mark.parametrize("dtype,heads,ps,pre,ext,mod", [
+    (BF, (4, 2, 64), 16, [0, 33, 100, 16], [1, 9, 33, 64], dict()),
+    (HF, (3, 1, 128), 1, [1, 31, 900, 63], [5, 2, 4, 5], dict(slopes=True)),
+    (BF, (8, 1, 128), 16, [2000, 5], [64, 3], dict(softcap=20.0)),
+    (HF, (2, 2, 64), 5, [700], [8], dict()),
+])
+def test_tree_attention_in_a_window(dtype, heads, ps, pre, ext, mod, window):
+    """A window counts positions, so nodes of one depth leave it together: windows shorter than a tree is deep drop ancestors."""
+    c = Case(10, dtype, heads, ps, pre, ext)
+    parents = trees(11, ext[:-1]) + [list(range(-1, ext[-1] - 1))]                                    # (the last one a chain)
+    kw = dict(mod, window=window)
+    if "slopes" in kw:
+        kw["slopes"] = slopes_of(c.Hq)
+    ref = want(c, parents, **kw)
+    if "slopes" in kw:
+        kw["slopes"] = kw["slopes"].to(DEV)
+    check(attn(c, prepare(c, parents), **kw), *ref)
 
 
 def test_siblings_do_not_leak():
