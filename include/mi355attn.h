@@ -312,7 +312,7 @@ int m355_tree_prepare(int32_t *page_table, int64_t pt_row_stride, int32_t pt_row
  *     logprobs[t, g] = log p(tokens[t, g])   for `given` tokens a row (int64 [T, given]; an id outside [0, V): -inf);
  *     entropy[t] = -sum p log p;
  *     top_ids[t, :] = the top_k largest logits' ids, largest first, the lower id first among equals; top_logprobs their log p.
- * Sums in fp32.  Logits of -inf count as probability 0; a row with NaN, +inf or nothing above -inf gives NaN.
+ * Sums in fp32.  Logits of -inf count as probability 0; a row with NaN, +inf or nothing above -inf gives NaN, whatever the ids.
  * top_k <= min(V, M355_MAX_TOP_LOGPROBS).  workspace: m355_token_logprobs_workspace_bytes bytes, 256-byte aligned, may be NULL
  * where that is 0; calls that overlap need one each. */
 #define M355_MAX_TOP_LOGPROBS 64

@@ -105,6 +105,16 @@ def test_tokens_outside_the_vocabulary():
     check(x, torch.tensor([-1, 100, 2 ** 40]), 0)
 
 
+def test_ids_outside_where_a_row_has_no_distribution():
+    """The row's NaN comes first, whatever the id."""
+    from mi355_attn import ops
+    x = torch.zeros((4, 50))
+    x[0], x[1, 7], x[2, 3] = float("-inf"), float("nan"), float("inf")
+    r = ops.token_logprobs(x.to(DEV), torch.tensor([[50, 1], [-1, 7], [2 ** 40, 3], [50, 0]], device=DEV), top_k=2)
+    assert r.logprobs[:3].isnan().all() and r.entropy[:3].isnan().all()
+    assert r.logprobs[3, 0] == float("-inf") and torch.isfinite(r.logprobs[3, 1])
+
+
 def test_rows_of_any_alignment():
     g = torch.Generator().manual_seed(3)
     for dtype in (torch.bfloat16, torch.float32):
