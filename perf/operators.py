@@ -218,16 +218,12 @@ def prepare(case, seed):
 
 
 # ------------------------------------------------------------------------------------------------ the framework's operators
-_imported = []
-
-
 def _ops():
-    """The framework's operators, imported once as a program does."""
-    if not _imported:
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mini-sglang_amd"))
-        from mi355_attn import ops
-        _imported.append(ops)
-    return _imported[0]
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mini-sglang_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from mi355_attn import ops
+    return ops
 
 
 def _run_own(s):
