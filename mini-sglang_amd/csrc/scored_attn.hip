@@ -58,7 +58,7 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 // (16 requests of 20 000 to 32 768 tokens, 222 MB: 40.6 us, 5.5 TB/s; with four waves 49.8, with one 58.7).  More rows go to
 // the other kernel: with 32 rows here, 16 requests of 2 250 tokens took 45 us against 29.
 // ------------------------------------------------------------------------------------------------------------------------
-constexpr int kFewRows = 16, kFewWaves = 2, kWideRows = 128;
+constexpr int kFewWaves = 2;
 constexpr int kFewSlots = 1024;                       // tokens whose pool slots are in LDS at a time
 
 enum { kPlain, kCapped, kBiased };                         // what scores go through: the scale alone, a cap, distances (capped or not)
@@ -765,41 +765,6 @@ static int shift_of(int32_t x) {
     int s = 0;
     while ((1 << s) < x) ++s;
     return s;
-}
-
-// How a call is cut, from its sizes alone (so that the workspace query and the launch agree).  The rows a request brings choose the
-// kernel.  Keys are split where there are fewer (request, kv head, row block) units than twice the workgroups that the chip
-// holds at once; find_share then lays out the parts.  A part is at least 256 keys (128 in the few-row kernel), or a sixteenth of the
-// request where that is shorter: a single short request is a matter of latency (8 nodes over 700 tokens: 64 keys 9.8 + 4.2 us,
-// 128 keys 13.4 + 3.5, 256 keys 15.6 + 3.8; over 4 250 tokens: 256 keys 12.3 + 4.8, 128 keys 11.8 + 6.3).
-struct ScoredCut { bool wide; int32_t blocks, slots, max_parts; int64_t grid, part_bytes, bytes; };
-static ScoredCut scored_cut(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int32_t D, int64_t ext, int64_t max_len) {
-    constexpr int64_t kCus = 256;
-    ScoredCut c = {};
-    const int64_t G = Hq / Hkv;
-    if (ext > T) ext = T;
-    const int64_t rows = ext * G, rb = rows > kFewRows ? kWideRows : kFewRows;
-    c.wide = rows > kFewRows;
-    c.blocks = (int32_t)((rows + rb - 1) / rb);
-    // workgroups a CU holds: two by the LDS at head_dim 128, three by the registers and four by the LDS at 64 (16 draft trees over
-    // 500 to 4 000 tokens, wide, two a CU: 47 + 8 us; parts for one a CU: 62 + 6)
-    const int64_t slots = kCus * (D == 128 ? 2 : (c.wide ? 3 : 4));
-    // (a ragged batch has fewer row blocks than its longest request suggests)
-    int64_t blocks = B * c.blocks;
-    const int64_t packed = (T * G + rb - 1) / rb + B;
-    if (packed < blocks) blocks = packed;
-    c.grid = B * Hkv * c.blocks;
-    // (find_share reads 64 requests at a time: 250 requests of 63 to 2047 tokens on one kv head take 53.9 us whole and 32.3 + 4.3 in
-    // parts, 500 requests 64.2 and 64.8 + 4.5)
-    if (blocks * Hkv >= 2 * slots || max_len <= 64 || B > 256) return c;
-    c.slots = (int32_t)slots;
-    const int64_t units = blocks * Hkv, full = (int64_t)full_parts((float)slots, (float)units, !c.wide);
-    const int64_t low = Hkv & -Hkv, rounding = c.blocks > 1 ? 8 / (low < 8 ? low : 8) / 2 * units : 0;
-    c.max_parts = (int32_t)(full + units + rounding + 16);
-    c.grid = c.max_parts;
-    c.part_bytes = c.max_parts * rb * (D + 4) * (int64_t)sizeof(float);
-    c.bytes = c.part_bytes + T * Hq * (int64_t)sizeof(int2);
-    return c;
 }
 
 // what both entry points refuse

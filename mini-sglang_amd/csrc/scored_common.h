@@ -77,15 +77,13 @@ __device__ __forceinline__ T lane_value(T x, int lane) {
 
 // Splits follow the batch, which the host does not know: every wave reads the requests' lengths (one per lane) and lays the work
 // out for itself, the same way in all of them.
-//   work  W = sum over requests of row blocks x keys x kv heads; a part holds at most size = W / full_parts keys
-//   parts nsp = ceil(keys / size) per request, all of one length: full_parts + units at most, which sizes grid and workspace
+//   work  W = sum over requests of row blocks x keys x kv heads; a part holds at most size = W / full_parts keys (part_size)
+//   parts nsp = ceil(keys / size) per request, all of one length: full_parts + units at most, and what rounding to whole rounds of the 8
+//   XCDs adds (request_parts), which sizes grid and workspace
 // Workgroups are numbered request by request, so those with nothing to do come last.  A workgroup that only finds out that it is idle
 // still waits for a place and holds it for 2 us: with idle ones in between, the others started up to 40 us late.
-// Row blocks of one (request, kv head, part) lie 8 apart: on one XCD, whose L2 then reads their keys once.  Their parts come in
-// whole rounds of the 8 XCDs where there are that many (61 to 72 workgroups an XCD instead of 64 cost a second round: 73 us for 58).
 template <int RB, bool FEW>
 __device__ __forceinline__ Share find_share(const ScoredParams& p) {
-    constexpr int32_t shortest_max = FEW ? 128 : 256, shortest_min = FEW ? 128 : 64;     // keys of a part: scored_cut
     const int lane = threadIdx.x & 63;
     struct Req { ReqSpan r; int32_t blocks, keys, row; };
     auto load = [&](int b) {                           // everything a share needs of a request, in one round of loads
@@ -107,30 +105,20 @@ __device__ __forceinline__ Share find_share(const ScoredParams& p) {
     }
     work *= (float)p.Hkv;
     units *= (float)p.Hkv;
-    const int32_t size = (int32_t)fminf(work / full_parts((float)p.slots, units, FEW), 1e9f) + 1;
+    const int32_t size = part_size(work, units, (float)p.slots, FEW);
     int32_t at = (int32_t)blockIdx.x, part0 = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         const Req q = b0 ? load(b0 + lane) : first;
-        const int32_t least = imax(size, imax(shortest_min, imin(shortest_max, q.keys / 16)));
-        int32_t nsp = imax(1, (q.keys + least - 1) / least);
-        const bool rounds = q.blocks > 1 && nsp * p.Hkv >= 8;
-        if (rounds) {                                  // the nearest number of parts that gives whole rounds
-            const int32_t step = 8 / imin(p.Hkv & -p.Hkv, 8);
-            nsp = imax(step, (nsp + step / 2) / step * step);
-        }
-        const int32_t items = nsp * p.Hkv * q.blocks, parts = nsp * p.Hkv * q.blocks;
-        const int32_t items_to = wave_sums(items), parts_to = wave_sums(parts);
+        const int32_t nsp = request_parts(q.keys, q.blocks, size, p.Hkv, FEW);
+        const int32_t items = nsp * p.Hkv * q.blocks, items_to = wave_sums(items);       // (a workgroup a part)
         const unsigned long long past = __ballot(at < items_to);
         if (past) {
             const int k = __builtin_ctzll(past);       // the request of this workgroup, in lane k
             const int32_t i = at - lane_value(items_to - items, k), blocks = lane_value(q.blocks, k), n = lane_value(nsp, k);
             Share s;
-            int32_t u = i;
-            s.rb = 0;
-            if (blocks > 1) {
-                if (n * p.Hkv >= 8) { const int32_t y = i >> 3; s.rb = y % blocks; u = (y / blocks) * 8 + (i & 7); }
-                else { s.rb = i % blocks; u = i / blocks; }
-            }
+            const PartItem it = part_item(i, blocks, n, p.Hkv);
+            const int32_t u = it.u;
+            s.rb = it.rb;
             s.any = true;
             // the kv head turns with part and request: an XCD should not read one head's column of the pools only (8 heads, 8 XCDs)
             s.sp = u / p.Hkv;
@@ -138,14 +126,14 @@ __device__ __forceinline__ Share find_share(const ScoredParams& p) {
             s.h = blocks > 1 ? u % p.Hkv : (u + s.sp + s.b) % p.Hkv;
             s.nsp = n;
             s.chunk = ((lane_value(q.keys, k) + n - 1) / n + 63) & ~63;
-            s.part0 = part0 + lane_value(parts_to - parts, k) + (s.rb * p.Hkv + s.h) * n;
+            s.part0 = part0 + lane_value(items_to - items, k) + (s.rb * p.Hkv + s.h) * n;
             s.r = {lane_value(q.r.q0, k), lane_value(q.r.E, k), lane_value(q.r.P, k), lane_value(q.r.L, k)};
             s.pt_row = p.page_table + (int64_t)lane_value(q.row, k) * p.pt_stride;
-            if (s.part0 + n > p.max_parts) s.any = false;              // (only lengths that contradict T get here)
+            if (s.part0 + n > p.max_parts) s.any = false;              // (only cu_q that contradicts the call's bounds gets here)
             return s;
         }
         at -= lane_value(items_to, 63);
-        part0 += lane_value(parts_to, 63);
+        part0 += lane_value(items_to, 63);
     }
     Share none = {};
     return none;

@@ -54,12 +54,83 @@ M355_HD int32_t pool_slot(int32_t page, int32_t ps, int32_t offset, int64_t S) {
     return (int32_t)s;
 }
 
+// ---- Parts.  Keys are cut into parts where there are too few (request, kv head, row block) units for the chip.  The host sizes grid
+// and workspace from the call's bounds (scored_cut), the device lays the parts out from the batch's own lengths (find_share); both by
+// these functions, so that no batch within its bounds can want more parts than are reserved.
+constexpr int32_t kFewRows = 16, kWideRows = 128;                      // rows of a workgroup in the two kernels
+
 // Full parts that `units` units of work are cut into for `slots` workgroups: every unit ends in a part that is half full on average,
 // so the rest would run at once; at least half the slots, where the units alone nearly fill them.  The single-token kernel, which
 // memory alone bounds, keeps a few more places free for workgroups without work.
 M355_HD float full_parts(float slots, float units, bool few) {
     const float rest = slots - (few ? 0.75f : 0.5f) * units;
     return rest > 0.5f * slots ? rest : 0.5f * slots;
+}
+
+// keys of a full part; work: sum over units of their keys
+M355_HD int32_t part_size(float work, float units, float slots, bool few) {
+    const float size = work / full_parts(slots, units, few);
+    return (int32_t)(size < 1e9f ? size : 1e9f) + 1;
+}
+
+// Workgroups of one (request, kv head, part) lie 8 apart (part_item): its parts come in whole rounds of the 8 XCDs, `step` of them at
+// a time for these kv heads.
+M355_HD int32_t round_step(int32_t Hkv) { return 8 / imin(Hkv & -Hkv, 8); }
+
+// Parts of each unit of a request: ceil(keys / size) of one length, none shorter than scored_cut says; several row blocks take the
+// nearest number that gives whole rounds (61 to 72 workgroups an XCD instead of 64 cost a second round: 73 us for 58).  Rounding adds
+// step / 2 parts at most, which is what scored_cut reserves: a number below step / 2 stays as it is, it would grow up to eightfold.
+M355_HD int32_t request_parts(int32_t keys, int32_t blocks, int32_t size, int32_t Hkv, bool few) {
+    const int32_t shortest_max = few ? 128 : 256, shortest_min = few ? 128 : 64;
+    const int32_t least = imax(size, imax(shortest_min, imin(shortest_max, keys / 16)));
+    const int32_t nsp = imax(1, (keys + least - 1) / least), step = round_step(Hkv);
+    return blocks > 1 && nsp * Hkv >= 8 && nsp >= step / 2 ? (nsp + step / 2) / step * step : nsp;
+}
+
+// Workgroup i of a request with n parts a unit: its row block, and u = part * kv heads + kv head.  In whole rounds the row blocks of one
+// u lie 8 apart, on one XCD, whose L2 then reads their keys once; otherwise they lie side by side.
+struct PartItem { int32_t rb, u; };
+M355_HD PartItem part_item(int32_t i, int32_t blocks, int32_t n, int32_t Hkv) {
+    if (blocks <= 1) return {0, i};
+    if (n * Hkv % 8) return {i % blocks, i / blocks};
+    const int32_t y = i >> 3;
+    return {y % blocks, (y / blocks) * 8 + (i & 7)};
+}
+
+// How a call is cut, from its sizes alone (so that the workspace query and the launch agree).  The rows a request brings choose the
+// kernel.  Keys are split where there are fewer (request, kv head, row block) units than twice the workgroups that the chip
+// holds at once; find_share then lays out the parts.  A part is at least 256 keys (128 in the few-row kernel), or a sixteenth of the
+// request where that is shorter: a single short request is a matter of latency (8 nodes over 700 tokens: 64 keys 9.8 + 4.2 us,
+// 128 keys 13.4 + 3.5, 256 keys 15.6 + 3.8; over 4 250 tokens: 256 keys 12.3 + 4.8, 128 keys 11.8 + 6.3).
+struct ScoredCut { bool wide; int32_t blocks, slots, max_parts; int64_t grid, part_bytes, bytes; };
+inline ScoredCut scored_cut(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int32_t D, int64_t ext, int64_t max_len) {
+    constexpr int64_t kCus = 256;
+    ScoredCut c = {};
+    const int64_t G = Hq / Hkv;
+    if (ext > T) ext = T;
+    const int64_t rows = ext * G, rb = rows > kFewRows ? kWideRows : kFewRows;
+    c.wide = rows > kFewRows;
+    c.blocks = (int32_t)((rows + rb - 1) / rb);
+    // workgroups a CU holds: two by the LDS at head_dim 128, three by the registers and four by the LDS at 64 (16 draft trees over
+    // 500 to 4 000 tokens, wide, two a CU: 47 + 8 us; parts for one a CU: 62 + 6)
+    const int64_t slots = kCus * (D == 128 ? 2 : (c.wide ? 3 : 4));
+    // (a ragged batch has fewer row blocks than its longest request suggests)
+    int64_t blocks = B * c.blocks;
+    const int64_t packed = (T * G + rb - 1) / rb + B;
+    if (packed < blocks) blocks = packed;
+    c.grid = B * Hkv * c.blocks;
+    // (find_share reads 64 requests at a time: 250 requests of 63 to 2047 tokens on one kv head take 53.9 us whole and 32.3 + 4.3 in
+    // parts, 500 requests 64.2 and 64.8 + 4.5)
+    if (blocks * Hkv >= 2 * slots || max_len <= 64 || B > 256) return c;
+    c.slots = (int32_t)slots;
+    // full parts, one more a unit that is not full, and what rounding adds
+    const int64_t units = blocks * Hkv, full = (int64_t)full_parts((float)slots, (float)units, !c.wide);
+    const int64_t rounding = c.blocks > 1 ? round_step((int32_t)Hkv) / 2 * units : 0;
+    c.max_parts = (int32_t)(full + units + rounding + 16);
+    c.grid = c.max_parts;
+    c.part_bytes = c.max_parts * rb * (D + 4) * (int64_t)sizeof(float);
+    c.bytes = c.part_bytes + T * Hq * 2 * (int64_t)sizeof(int32_t);
+    return c;
 }
 
 // A request's rows as the kernels use them: q rows q0 .. q0 + E, positions P + j, L cached tokens - whatever the device
