@@ -92,7 +92,7 @@ __device__ __forceinline__ Share find_share(const ScoredParams& p) {
         const int64_t row = p.page_table_ids[at];
         q.r = load_span(p, at);
         q.row = (int32_t)(row < 0 ? 0 : (row >= p.pt_rows ? p.pt_rows - 1 : row));
-        q.blocks = b < p.B ? (q.r.E * p.G + RB - 1) / RB : 0;
+        q.blocks = b < p.B ? row_blocks(q.r.E, p.G, RB, p.blocks) : 0;
         q.keys = p.window > 0 ? imin(q.r.L, imin(p.window, 0x3fffffff) + (p.mask ? q.r.E : RB)) : q.r.L;
         return q;
     };

@@ -67,6 +67,10 @@ M355_HD float full_parts(float slots, float units, bool few) {
     return rest > 0.5f * slots ? rest : 0.5f * slots;
 }
 
+// Row blocks of a request with E rows of G heads, `most` of them: a request with more rows than the call's bound promised keeps to the
+// blocks that were reserved for it and takes nobody else's.
+M355_HD int32_t row_blocks(int32_t E, int32_t G, int32_t block_rows, int32_t most) { return imin((E * G + block_rows - 1) / block_rows, most); }
+
 // keys of a full part; work: sum over units of their keys
 M355_HD int32_t part_size(float work, float units, float slots, bool few) {
     const float size = work / full_parts(slots, units, few);

@@ -26,7 +26,7 @@ extern "C" int layout(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, 
     float work = 0.f, units = 0.f;
     std::vector<int32_t> blocks(B);
     for (int b = 0; b < B; ++b) {
-        blocks[b] = (E[b] * G + rb - 1) / rb;
+        blocks[b] = row_blocks(E[b], G, rb, c.blocks);
         work += (float)blocks[b] * (float)K[b];
         units += (float)blocks[b];
     }
@@ -94,6 +94,32 @@ def test_no_batch_wants_more_parts_than_are_reserved(layout, Hkv):
         assert nbytes == _lib.load().m355_scored_workspace_bytes(B, sum(ext), G * Hkv, Hkv, D, max(ext), max(keys))
         split += reserved > 0
     assert split > 40
+
+
+@pytest.mark.parametrize("promised", [1, 4, 40])
+def test_rows_past_the_promise_take_no_other_requests_parts(layout, promised):
+    """max_extend_len below what some requests bring: those rows may be left out, the parts of all others are still reserved."""
+    rng = random.Random(promised)
+    for heads in ((8, 1, 64), (8, 2, 128), (9, 3, 64), (32, 8, 128)):
+        for _ in range(100):
+            B = rng.randint(2, 60)
+            ext = [rng.choice([promised, 500]) for _ in range(B)]
+            code, reserved, wanted, _ = layout(*heads, ext, [e + rng.randint(100, 3000) for e in ext], hint_ext=promised)
+            assert code == 0, (heads, ext, wanted, reserved)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,promised", [((8, 1, 64), 2), ((8, 2, 128), 4), ((4, 1, 64), 40)])
+def test_rows_past_the_promise_leave_other_requests_alone(heads, promised):
+    """The longest requests stand first: what they bring beyond the promise costs no later request its rows."""
+    ext = [200] * 12 + [promised] * 12
+    c = Case(63, BF, heads, 16, [700] * 24, ext)
+    from mi355_attn import ops
+    got = ops.scored_attn(c.q.reshape(c.T, -1).to(DEV), c.pool(c.k), c.pool(c.v), c.table.to(DEV), c.rows.to(DEV), torch.tensor(c.len, device=DEV), 16, c.Hq,
+                          max(c.len), prefix_lens=torch.tensor(c.pre, device=DEV), cu_q=torch.tensor(c.cu, dtype=torch.int32, device=DEV),
+                          max_extend_len=promised, out=torch.full((c.T, c.Hq * c.D), float("nan"), dtype=BF, device=DEV)).view(c.T, c.Hq, c.D)
+    rows = list(range(promised))
+    check(got[[c.cu[b] + j for b in range(24) for j in rows]], *c.want(rows=rows))
 
 
 @pytest.mark.gpu
