@@ -36,9 +36,8 @@ __device__ __forceinline__ ReqSpan load_span(const ScoredParams& p, int b) {
         return req_span(b, b + 1, L - 1, L, p.T, tokens);
     }
     const int64_t q0 = p.cu_q[b], q1 = p.cu_q[b + 1], P = p.prefix_lens[b];
-    return req_span(q0, q1, P, p.seq_lens ? p.seq_lens[b] : P + (q1 - q0), p.T, tokens);
+    return p.seq_lens ? req_span(q0, q1, P, p.seq_lens[b], p.T, tokens) : tree_span(q0, q1, P, p.T, tokens);
 }
-
 
 __device__ __forceinline__ const int32_t* table_row(const ScoredParams& p, int b) {
     int64_t r = p.page_table_ids[b];

@@ -151,5 +151,11 @@ M355_HD ReqSpan req_span(int64_t q0, int64_t q1, int64_t P, int64_t L, int64_t T
     if (q0 > T) { q0 = T; q1 = T; }
     return {(int32_t)q0, (int32_t)(q1 - q0), (int32_t)P, (int32_t)L};
 }
+// The same for a tree behind a prefix of P tokens: its tokens end with the last node that has a row, so key - P is a node of the request's
+// own rows wherever it is used as one.
+M355_HD ReqSpan tree_span(int64_t q0, int64_t q1, int64_t P, int64_t T, int64_t table_tokens) {
+    const ReqSpan r = req_span(q0, q1, P, 0, T, table_tokens);
+    return req_span(q0, q1, P, (int64_t)r.P + r.E, T, table_tokens);
+}
 
 }  // namespace m355
