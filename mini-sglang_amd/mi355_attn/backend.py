@@ -68,8 +68,10 @@ def _drop_pad(o: torch.Tensor, Hkv: int, G: int, Gp: int, D: int) -> torch.Tenso
 
 
 def _modifiers(layer) -> dict:
-    """The score modifiers of a layer as ops.scored_attn takes them; a reference layer has none."""
-    return {"softcap": getattr(layer, "logit_cap", 0.0), "slopes": getattr(layer, "slopes", None), "window": getattr(layer, "window", 0)}
+    """The score modifiers of a layer as ops.scored_attn takes them; a reference layer has none, and its scale is not used."""
+    cap, slopes, window = getattr(layer, "logit_cap", 0.0), getattr(layer, "slopes", None), getattr(layer, "window", 0)
+    return {"softcap": cap, "slopes": slopes, "window": window,
+            "scale": getattr(layer, "score_scale", None) if cap or window or slopes is not None else None}
 
 
 def _masks(batch) -> dict:
