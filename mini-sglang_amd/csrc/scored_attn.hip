@@ -48,6 +48,12 @@ __device__ __forceinline__ BlockRange join16(BlockRange a) {
 // softmax(-inf everywhere so far): the difference of two -inf would be NaN
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
 
+// Weights go into the second product rounded to the element type.  Half precision keeps 11 bits of a weight down to 2^-14 and nothing
+// below 2^-25, which 100 000 keys make a sum of 2^-8 of: there the weights are 2^7 times as large, which drops out of the
+// softmax, and with the lazy maximum's 2^8 they end at 2^15.  What is lost is then 2^-32 of the largest weight a key at most.
+template <bool F16>
+constexpr float kLift = F16 ? 7.f : 0.f;
+
 // ------------------------------------------------------------------------------------------------------------------------
 // Up to 16 rows (single tokens): a workgroup takes the rows of one (request, kv head) and one split of the keys.  Its two waves
 // walk tiles of 32 keys on their own (tile 2 i + wave), each with its own two-stage LDS ring filled by LDS-DMA: K and V are read once,
@@ -210,11 +216,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void scored_few_kernel(const Scored
         lane_pair<32>(mx, a, c);
         mx = fmaxf(a, c);
         if constexpr (!MOD) mx *= p.scale_log2;
-        // the running maximum moves only when beaten by 2^kLazyMax: rescaling is rare, weights stay below 2^kLazyMax
+        // the running maximum moves only when beaten by 2^kLazyMax: rescaling is rare, weights stay below
+        // 2^(kLazyMax + kLift)
         const float m_new = mx > m_run + kLazyMax ? mx : m_run;
         const float alpha = m_new == m_run ? 1.f : exp2_fast(m_run - m_new);
         m_run = m_new;
-        const float mu = finite_max(m_new);
+        const float mu = finite_max(m_new) - kLift<F16>;
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) { s[i] = exp2_fast(MOD ? s[i] - mu : fmaf(s[i], p.scale_log2, -mu)); sum += s[i]; }
@@ -529,7 +536,7 @@ __global__ __launch_bounds__(256, 2) void scored_wide_kernel(const ScoredParams 
         return alpha;
     };
     auto exp_pack = [&](f32x16& s, bf16x8 (&pf)[2]) {
-        const float mu = finite_max(m_run);
+        const float mu = finite_max(m_run) - kLift<F16>;
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) { s[i] = exp2_fast(fmaf(s[i], unit, -mu)); sum += s[i]; }
