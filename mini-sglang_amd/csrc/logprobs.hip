@@ -175,7 +175,7 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(const Logpr
 #pragma unroll
         for (int v = 0; v < NV; ++v) cur[v] = next[v];
         if (blk + 1 < b1) fetch(blk + 1);
-        // index of element e: i0 + (e / VE) 256 VE + e % VE
+        // index of element e: i0 + (e / VE) kThreads VE + e % VE
         const int32_t i0 = (blk * NV * kThreads + tid) * VE - skip;
         auto inside = [&](int e) { const int32_t i = i0 + (e / VE) * kThreads * VE + e % VE; return i >= 0 && i < p.V; };
         if (blk == 0 || (blk + 1) * NV * kThreads >= n_vec) {

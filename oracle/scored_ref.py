@@ -76,8 +76,9 @@ def logprobs_ref(logits, tokens, top_k, temperature):
 
 
 def logprobs_bound(logits, temperature):
-    """Bound per row on log S, and the rounding of (x - max) / temperature: a thread adds V / 256 terms at most one after the
-    other and 256 partial sums pairwise; an exponential is off by its argument's rounding, |d| 2^-23 weighted by e^d / S, which is
-    log V 2^-23 at most, and two units of its own."""
+    """Bound per row on log S, and the rounding of (x - max) / temperature, for any layout in which a thread adds V / 256 terms at most
+    one after the other and the partial sums meet pairwise; an exponential is off by its argument's rounding, |d| 2^-23 weighted by
+    e^d / S, which is log V 2^-23 at most, and two units of its own.  The kernel's threads add V / 512 at most, fewer where rows are
+    split: tests/test_logprobs_sums.py holds it to that."""
     V = logits.shape[1]
     return (V / 256 + 64) * 2.0 ** -24
