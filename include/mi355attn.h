@@ -281,7 +281,7 @@ typedef struct M355ScoredArgs {
     int64_t pool_row_stride, pool_rows; /* 0: contiguous;  token rows of the pools, < 2^31                */
     int64_t pt_row_stride, workspace_bytes;
     int32_t pt_rows, pt_cols, B, T;
-    int32_t max_extend_len;          /* >= the longest cu_q[b+1] - cu_q[b]: rows past it may be left out  */
+    int32_t max_extend_len;          /* >= the longest cu_q[b+1] - cu_q[b]: rows past it mean nothing     */
     int32_t max_seq_len_hint;        /* >= the longest request, for the choice of the launch              */
     int32_t Hq, Hkv, D, page_size, window, mask_words, dtype;
     float scale, softcap;
