@@ -298,19 +298,24 @@ class Batch:
             raise RuntimeError(f"a tree would reach token {max(lens)}: more than the page table's {width} columns (max_context_len)")
         if sum(-(-n // ps) - -(-p // ps) for n, p in zip(lens, held)) > self.kvcache.available_page_num():
             raise RuntimeError("KV pool exhausted by draft trees (call check_decode_mem / retract_decode first)")
+        mode = self.mode
         self._begin(Mode.TREE)
-        self._tree_pages = self.kvcache.allocate_pages_prefill(lens, held)
-        self._tree_parents = [list(p) for p in parents]
-        self.tree_lens_host = lens
-        cu, off = np.concatenate([[0], np.cumsum(nodes)]), np.concatenate([[0], np.cumsum([len(p) for p in self._tree_pages])])
-        B, T, n_new = len(nodes), int(cu[-1]), int(off[-1])
-        i32 = _h2d(np.concatenate([np.concatenate(self._tree_parents), cu, off, np.concatenate([np.asarray(p, dtype=np.int64) for p in self._tree_pages])])
-                   .astype(np.int32), self.device)
-        self.input_ids = _h2d(np.concatenate([np.asarray(i, dtype=np.int64) for i in draft_ids]), self.device)
-        self.output_ids = None
-        self.tree = ops.tree_prepare(self.page_manager.page_table, self.page_table_ids, self.seq_lens, i32[:T], i32[T:T + B + 1], ps, max(nodes),
-                                     new_pages=i32[T + 2 * (B + 1):T + 2 * (B + 1) + n_new], new_page_off=i32[T + B + 1:T + 2 * (B + 1)])
-        self.positions, self.out_cache_loc, self.cu_q, self.row_of_token = self.tree.positions, self.tree.out_cache_loc, self.tree.cu_q, None
+        pages = self.kvcache.allocate_pages_prefill(lens, held)
+        try:
+            cu, off = np.concatenate([[0], np.cumsum(nodes)]), np.concatenate([[0], np.cumsum([len(p) for p in pages])])
+            B, T, n_new = len(nodes), int(cu[-1]), int(off[-1])
+            i32 = _h2d(np.concatenate([np.concatenate(parents), cu, off, np.concatenate([np.asarray(p, dtype=np.int64) for p in pages])])
+                       .astype(np.int32), self.device)
+            input_ids = _h2d(np.concatenate([np.asarray(i, dtype=np.int64) for i in draft_ids]), self.device)
+            tree = ops.tree_prepare(self.page_manager.page_table, self.page_table_ids, self.seq_lens, i32[:T], i32[T:T + B + 1], ps, max(nodes),
+                                    new_pages=i32[T + 2 * (B + 1):T + 2 * (B + 1) + n_new], new_page_off=i32[T + B + 1:T + 2 * (B + 1)])
+        except Exception:                                   # (another current device, for one): no tree, and nothing of the pool is kept
+            self.kvcache._free_pages([p for some in pages for p in some])
+            self.mode = mode
+            raise
+        self.tree, self.tree_lens_host, self.input_ids, self.output_ids = tree, lens, input_ids, None
+        self._tree_parents, self._tree_pages = [list(p) for p in parents], pages
+        self.positions, self.out_cache_loc, self.cu_q, self.row_of_token = tree.positions, tree.out_cache_loc, tree.cu_q, None
 
     def commit_tree(self, accepted: List[List[int]]) -> None:
         """Ends a verification step: request b keeps the nodes accepted[b], a path from a root downwards (may be empty).  Their

@@ -73,3 +73,17 @@ def test_scaled_capped_layers_through_the_backend(scale):
     batch.output_ids = torch.zeros(1, dtype=torch.int64, device=DEV)
     batch.prepare_for_decode()
     step(1, [([*range(n + 3)],) * 2 + (n + 2,)])
+
+
+def test_a_tree_that_cannot_be_prepared_takes_no_pages(monkeypatch):
+    """The metadata launch refuses (here for want of a GPU): pages and mode are as they were, and the next step can begin."""
+    import mi355_attn as m
+    from test_speculate import _cpu_batch
+    b, kv = _cpu_batch()
+    b.mode, b.seq_lens, b.page_table_ids = m.Mode.DECODE, torch.tensor([6, 8]), torch.tensor([0, 1])
+    before, table = sorted(kv.free_pages), b.page_manager.page_table.clone()
+    for _ in range(8):                                                     # (more often than the pool has room for)
+        with pytest.raises(RuntimeError, match="GPU"):
+            b.prepare_for_tree([[1] * 9, [2] * 5], [list(range(-1, 8)), [-1] * 5])
+        assert sorted(kv.free_pages) == before and b.tree is None and b.mode is m.Mode.DECODE
+    assert torch.equal(b.page_manager.page_table, table)
