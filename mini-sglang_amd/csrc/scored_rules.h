@@ -83,7 +83,9 @@ M355_HD int32_t round_step(int32_t Hkv) { return 8 / imin(Hkv & -Hkv, 8); }
 
 // Parts of each unit of a request: ceil(keys / size) of one length, none shorter than scored_cut says; several row blocks take the
 // nearest number that gives whole rounds (61 to 72 workgroups an XCD instead of 64 cost a second round: 73 us for 58).  Rounding adds
-// step / 2 parts at most, which is what scored_cut reserves: a number below step / 2 stays as it is, it would grow up to eightfold.
+// step / 2 parts at most, which is what scored_cut reserves: a number below step / 2 stays as it is, it would grow up to eightfold (40/10
+// heads of 128, 20 requests of 64 rows over 1000 tokens: 54 us with one part, 94 with four; 9/3 heads of 64, 40 of 64 over 2000: 37
+// with three, 49 with eight).
 M355_HD int32_t request_parts(int32_t keys, int32_t blocks, int32_t size, int32_t Hkv, bool few) {
     const int32_t shortest_max = few ? 128 : 256, shortest_min = few ? 128 : 64;
     const int32_t least = imax(size, imax(shortest_min, imin(shortest_max, keys / 16)));
@@ -124,7 +126,8 @@ inline ScoredCut scored_cut(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int32
     if (packed < blocks) blocks = packed;
     c.grid = B * Hkv * c.blocks;
     // (find_share reads 64 requests at a time: 250 requests of 63 to 2047 tokens on one kv head take 53.9 us whole and 32.3 + 4.3 in
-    // parts, 500 requests 64.2 and 64.8 + 4.5)
+    // parts, 500 requests 64.2 and 64.8 + 4.5; lengths spread further than that were not measured: whole, the longest request is the
+    // launch's time)
     if (blocks * Hkv >= 2 * slots || max_len <= 64 || B > 256) return c;
     c.slots = (int32_t)slots;
     // full parts, one more a unit that is not full, and what rounding adds
