@@ -49,8 +49,8 @@ __device__ __forceinline__ BlockRange join16(BlockRange a) {
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
 
 // Weights go into the second product rounded to the element type.  Half precision keeps 11 bits of a weight down to 2^-14 and nothing
-// below 2^-25, which 100 000 keys make a sum of 2^-8 of: there the weights are 2^7 times as large, which drops out of the
-// softmax, and with the lazy maximum's 2^8 they end at 2^15.  What is lost is then 2^-32 of the largest weight a key at most.
+// below 2^-25, while 100 000 keys of that weight sum to 2^-8 of the best one's.  So in half precision all weights are 2^7 times as large,
+// which drops out of the softmax; with the lazy maximum's 2^8 they end at 2^15.  A key then loses 2^-32 of the best one's weight at most.
 template <bool F16>
 constexpr float kLift = F16 ? 7.f : 0.f;
 
